@@ -11,6 +11,7 @@ import os
 
 AM_DT_F32, AM_DT_BF16, AM_DT_F16, AM_DT_I8, AM_DT_I4, AM_DT_I32, AM_DT_I64, AM_DT_U32, AM_DT_U8 = range(9)
 AM_WF_F32, AM_WF_BF16, AM_WF_INT8, AM_WF_INT4 = range(4)
+AM_KV_PLAIN, AM_KV_MXFP4 = range(2)
 AM_PREFILL_SPLIT, AM_PREFILL_SILU_MUL, AM_PREFILL_QKV_ROPE_KV = 0, 1, 2
 AM_LOAD_STRICT_TENSOR_NAMES, AM_LOAD_REJECT_UNKNOWN_TENSORS, AM_LOAD_ALLOW_QUANTIZED_TENSORS = 1, 2, 4
 (AM_ROLE_QKV, AM_ROLE_O, AM_ROLE_GATE_UP, AM_ROLE_DOWN, AM_ROLE_LM_HEAD, AM_ROLE_Q, AM_ROLE_K, AM_ROLE_V,
@@ -81,6 +82,36 @@ class AttentionArgs(C.Structure):
                 ("head_dim", i64), ("capacity", i64), ("start_pos", i64), ("start_pos_dev", vp), ("batch", i64),
                 ("cache_batch_stride", i64), ("dtype", i32), ("num_splits", i32), ("workspace", vp),
                 ("workspace_bytes", i64), ("pages", C.POINTER(KvPages))]
+
+
+class QkNormRopeArgs(C.Structure):
+    _fields_ = [("q", vp), ("k", vp), ("q_out", vp), ("k_out", vp), ("rows", i64), ("hq", i64), ("hkv", i64),
+                ("head_dim", i64), ("q_stride", i64), ("k_stride", i64), ("q_out_stride", i64), ("k_out_stride", i64),
+                ("q_norm_w", vp), ("k_norm_w", vp), ("eps", f32), ("pos", vp), ("cos_tab", vp), ("sin_tab", vp),
+                ("max_pos", i64), ("dtype", i32)]
+
+
+class KvAppendArgs(C.Structure):
+    _fields_ = [("q", vp), ("k", vp), ("v", vp), ("q_out", vp), ("batch", i64), ("seq", i64), ("hq", i64), ("hkv", i64),
+                ("head_dim", i64), ("q_stride", i64), ("k_stride", i64), ("v_stride", i64), ("q_out_stride", i64),
+                ("q_norm_w", vp), ("k_norm_w", vp), ("eps", f32), ("cos_tab", vp), ("sin_tab", vp), ("max_pos", i64),
+                ("start_pos_dev", vp), ("seq_lens", vp), ("k_cache", vp), ("v_cache", vp), ("k_scales", vp),
+                ("v_scales", vp), ("capacity", i64), ("cache_batch_stride", i64), ("cache_format", i32), ("dtype", i32),
+                ("err_flag", vp), ("pages", C.POINTER(KvPages))]
+
+
+class Kv4ReadArgs(C.Structure):
+    _fields_ = [("k_codes", vp), ("k_scales", vp), ("v_codes", vp), ("v_scales", vp), ("k_out", vp), ("v_out", vp),
+                ("batch", i64), ("seq", i64), ("hkv", i64), ("head_dim", i64), ("capacity", i64),
+                ("cache_batch_stride", i64), ("start_pos_dev", vp), ("seq_lens", vp), ("out_dtype", i32),
+                ("pages", C.POINTER(KvPages))]
+
+
+class Kv4AttentionArgs(C.Structure):
+    _fields_ = [("q", vp), ("out", vp), ("k_codes", vp), ("k_scales", vp), ("v_codes", vp), ("v_scales", vp),
+                ("batch", i64), ("seq", i64), ("hq", i64), ("hkv", i64), ("head_dim", i64), ("capacity", i64),
+                ("cache_batch_stride", i64), ("start_pos_dev", vp), ("seq_lens", vp), ("scale", f32), ("dtype", i32),
+                ("workspace", vp), ("workspace_bytes", i64), ("pages", C.POINTER(KvPages))]
 
 
 class SiluMulArgs(C.Structure):
@@ -214,6 +245,11 @@ _SIGS = {
     "am_gfx950_attention_workspace_bytes": (i64, [i64, i64, i64, i64, i64, i64, i32]),
     "am_gfx950_attention_noalloc": (i32, [C.POINTER(AttentionArgs), vp]),
     "am_gfx950_attention_noalloc_max_bytes": (i64, []),
+    "am_gfx950_qk_norm_rope": (i32, [C.POINTER(QkNormRopeArgs), vp]),
+    "am_gfx950_kv_append": (i32, [C.POINTER(KvAppendArgs), vp]),
+    "am_gfx950_kv4_read": (i32, [C.POINTER(Kv4ReadArgs), vp]),
+    "am_gfx950_kv4_attention": (i32, [C.POINTER(Kv4AttentionArgs), vp]),
+    "am_gfx950_kv4_attention_workspace_bytes": (i64, [i64, i64, i64, i64, i64, i64]),
     "am_gfx950_silu_mul": (i32, [C.POINTER(SiluMulArgs), vp]),
     "am_gfx950_add": (i32, [C.POINTER(AddArgs), vp]),
     "am_gfx950_argmax": (i32, [C.POINTER(ArgmaxArgs), vp]),

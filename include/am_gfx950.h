@@ -293,6 +293,152 @@ int64_t am_gfx950_attention_workspace_bytes(int64_t batch, int64_t seq, int64_t 
 am_status_code am_gfx950_attention_noalloc(const am_gfx950_attention_args* args, void* hip_stream);
 int64_t am_gfx950_attention_noalloc_max_bytes(void);
 
+/* Per-head RMSNorm of queries and keys with the rotation in the same pass (models that
+ * norm q and k before RoPE; no reference OpType): with x one head's row of q (or k),
+ *   y = x * (mean(x^2) + eps)^-1/2 * w   (w NULL: y = x),   out = rotate(y, pos[row]),
+ * the split-half rotation of am_gfx950_rope with its tables; a row whose position lies
+ * outside [0, max_pos) is normed and not rotated.  fp32 (a sum of squares and a rotation
+ * of fp32 values), one rounding to dtype, so without gains it equals am_gfx950_rope.
+ * Rows may be strided: row i, head h of q starts at element i * q_stride + h * head_dim,
+ * so q and k may be views into the rows of one q|k|v product.  An output may be its own
+ * input with the same stride; otherwise the buffers must not overlap.  hq or hkv may be 0
+ * (its pointers are then unused).  head_dim: even, at most 1024; head_dim 64, 128 and 256
+ * take the vector kernel. */
+typedef struct am_gfx950_qk_norm_rope_args {
+  const void* q;
+  const void* k;
+  void* q_out;
+  void* k_out;
+  int64_t rows, hq, hkv, head_dim;
+  int64_t q_stride, k_stride, q_out_stride, k_out_stride; /* elements between rows */
+  const void* q_norm_w; /* [head_dim], dtype; NULL: no norm */
+  const void* k_norm_w;
+  float eps;            /* used with a gain */
+  const int64_t* pos;   /* device [rows] */
+  const float* cos_tab; /* [max_pos][head_dim/2], am_gfx950_rope_table */
+  const float* sin_tab;
+  int64_t max_pos;
+  int32_t dtype;        /* F32 / BF16 */
+} am_gfx950_qk_norm_rope_args;
+am_status_code am_gfx950_qk_norm_rope(const am_gfx950_qk_norm_rope_args* args, void* hip_stream);
+
+/* KV cache formats.  AM_KV_MXFP4 (head_dim 64 or 128) holds 4.25 bits a value: per row of
+ * one head, head_dim/2 bytes of E2M1 codes (low nibble = even dimension) in the code
+ * cache and head_dim/32 bytes of E8M0 scales, one per 32 dimensions, in the scale cache:
+ *   value = code * 2^(scale - 127), code in +-{0, 0.5, 1, 1.5, 2, 3, 4, 6}; scale 255: NaN
+ * (253 and 254, whose values would pass bf16, are never written and read as NaN too).
+ * Both caches have the layout of a plain cache with a row as their element:
+ * [hkv][capacity][row bytes] planes per sequence, or block pools
+ * [num_blocks][hkv][block_size][row bytes]; cache_batch_stride counts values (a sequence's
+ * planes start cache_batch_stride / 2 code bytes and / 32 scale bytes after the one before).
+ * Code and scale caches are 16-byte aligned, and without pages capacity is a multiple of
+ * 32 and cache_batch_stride one of 32 * head_dim.
+ * Writing a group x of 32: the scale is the smallest 2^e with max|x| < 7 * 2^e, e in
+ * [-127, 125], and every code the nearest to x / 2^e, ties to the even code, saturating
+ * at 6; so below 7 * 2^125 a value is off by at most half the step of its code.  A group
+ * that holds a NaN or an infinity gets scale 255 and reads as NaN. */
+typedef enum am_kv_cache_format {
+  AM_KV_PLAIN = 0, /* the activation dtype */
+  AM_KV_MXFP4 = 1
+} am_kv_cache_format;
+
+/* (Norm and) rotation of q and k and the cache write of k and v for a padded batch of
+ * sequences in one launch (RmsNorm per head, kRoPE, kKVCacheUpdate; rope_op.cpp:11-223,
+ * kvcache_update_op.cpp:50-138).  Row b * seq + s of q, k and v is position
+ * start_pos_dev[b] + s of sequence b, live for s < seq_lens[b] (NULL: all seq rows); rows
+ * behind it are not read, and their q_out and cache rows are left as they were.  q and k
+ * are normed where a gain is given and rotated as in am_gfx950_qk_norm_rope; q_out gets
+ * the rotated q and the cache the rotated k and v.  A live row whose position lies outside
+ * [0, capacity) writes no cache row, keeps q unrotated and sets *err_flag; a position
+ * whose block-table entry lies outside the pool writes no cache row and sets the pages'
+ * err_flag (err_flag when that is NULL).
+ * AM_KV_PLAIN holds k as am_gfx950_rope followed by am_gfx950_kv_update would (one
+ * rounding with a gain) and v's bits.  AM_KV_MXFP4 rounds k once, from a norm and rotation
+ * in 64 bits, so no code depends on the order of a sum.
+ * Strides and aliasing as in am_gfx950_qk_norm_rope (q_out may be q).  hq may be 0 (keys
+ * and values only).  Sequences must not share cache rows. */
+typedef struct am_gfx950_kv_append_args {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* q_out;
+  int64_t batch, seq, hq, hkv, head_dim;
+  int64_t q_stride, k_stride, v_stride, q_out_stride; /* elements between rows */
+  const void* q_norm_w; /* [head_dim], dtype; NULL: no norm */
+  const void* k_norm_w;
+  float eps;
+  const float* cos_tab; /* [max_pos][head_dim/2] */
+  const float* sin_tab;
+  int64_t max_pos;      /* at least capacity */
+  const int64_t* start_pos_dev; /* device [batch] */
+  const int32_t* seq_lens;      /* device [batch], or NULL */
+  void* k_cache;        /* planes or pools; AM_KV_MXFP4: codes */
+  void* v_cache;
+  uint8_t* k_scales;    /* AM_KV_MXFP4 only */
+  uint8_t* v_scales;
+  int64_t capacity, cache_batch_stride;
+  int32_t cache_format; /* am_kv_cache_format */
+  int32_t dtype;        /* q, k, v, gains: F32 / BF16 */
+  int32_t* err_flag;    /* optional */
+  const am_gfx950_kv_pages* pages; /* NULL: contiguous planes */
+} am_gfx950_kv_append_args;
+am_status_code am_gfx950_kv_append(const am_gfx950_kv_append_args* args, void* hip_stream);
+
+/* Rows of an AM_KV_MXFP4 cache back as values (exact in both output dtypes): row
+ * b * seq + s of k_out and v_out [batch * seq][hkv * head_dim] is position
+ * start_pos_dev[b] + s of sequence b for s < seq_lens[b] (NULL: all); rows behind it are
+ * left as they were.  A position outside [0, capacity) gives a zero row. */
+typedef struct am_gfx950_kv4_read_args {
+  const uint8_t* k_codes;
+  const uint8_t* k_scales;
+  const uint8_t* v_codes;
+  const uint8_t* v_scales;
+  void* k_out;
+  void* v_out;
+  int64_t batch, seq, hkv, head_dim, capacity, cache_batch_stride;
+  const int64_t* start_pos_dev; /* device [batch] */
+  const int32_t* seq_lens;      /* device [batch], or NULL */
+  int32_t out_dtype;            /* F32 / BF16 */
+  const am_gfx950_kv_pages* pages;
+} am_gfx950_kv4_read_args;
+am_status_code am_gfx950_kv4_read(const am_gfx950_kv4_read_args* args, void* hip_stream);
+
+/* OpType::kAttention (attention_op.cpp:11-169) over an AM_KV_MXFP4 cache: causal GQA for a
+ * padded batch.  q and out [batch * seq][hq * head_dim]; row b * seq + s, live for
+ * s < seq_lens[b] (NULL: all), sits at position start_pos_dev[b] + s and attends to cache
+ * positions up to it, below capacity: a row before position 0 has no keys and gives zeros,
+ * one past the cache has all of them.  Rows behind seq_lens[b] are left as they were.
+ * out = sum_t softmax_t(scale * q . K_t) V_t over the values that the cache stands for;
+ * q head h reads kv head h / (hq / hkv), at most 16 q heads per kv head; fp32 online
+ * softmax; the products take q as it is (bf16) or as three bf16 parts (fp32) and the
+ * probabilities as two or three, so neither adds to the one rounding of out.  Scores of
+ * which none exceeds minus infinity give zeros.  A NaN among a row's keys gives NaN (a NaN
+ * value only in its own 32 dimensions); what the cache holds past a row's keys does not
+ * matter.  q and out are 16-byte aligned.
+ * workspace: am_gfx950_kv4_attention_workspace_bytes(...) bytes, 16-byte aligned, whose
+ * first 16384 bytes must be zero before the first call and are left zero.  One workspace
+ * serves calls of any shapes in turn; calls that overlap on one workspace race.  The
+ * results do not depend on the scheduling of blocks. */
+typedef struct am_gfx950_kv4_attention_args {
+  const void* q;
+  void* out;
+  const uint8_t* k_codes;
+  const uint8_t* k_scales;
+  const uint8_t* v_codes;
+  const uint8_t* v_scales;
+  int64_t batch, seq, hq, hkv, head_dim, capacity, cache_batch_stride;
+  const int64_t* start_pos_dev; /* device [batch] */
+  const int32_t* seq_lens;      /* device [batch], or NULL */
+  float scale;                  /* of the scores; 0: 1/sqrt(head_dim) */
+  int32_t dtype;                /* q and out: F32 / BF16 */
+  void* workspace;
+  int64_t workspace_bytes;
+  const am_gfx950_kv_pages* pages;
+} am_gfx950_kv4_attention_args;
+am_status_code am_gfx950_kv4_attention(const am_gfx950_kv4_attention_args* args, void* hip_stream);
+int64_t am_gfx950_kv4_attention_workspace_bytes(int64_t batch, int64_t seq, int64_t hq, int64_t hkv,
+                                                int64_t head_dim, int64_t capacity);
+
 /* OpType::kSiluMul (silu_mul_op.cpp:32-61; formula const_eval_silu_mul.cpp:18-31). */
 typedef struct am_gfx950_silu_mul_args {
   const void* gate;
