@@ -46,6 +46,8 @@ struct Attn4Args {
   int32_t batch, seq, hq, hkv, G, qt, tiles, units, cap;
   int32_t slots;  // planned grid; 0: one piece per unit
   int32_t min_steps;
+  uint32_t tiles_inv;  // ceil(2^32 / tiles): unit / tiles by a multiplication (below 2^16 units)
+  int32_t g_inv;  // ceil(2^16 / G): c / G = (c * g_inv) >> 16 for a column c < 16
   float scale;  // of the scores, times log2(e)
 };
 
@@ -84,9 +86,13 @@ __device__ __forceinline__ int wave_scan_i(int v) {
 }
 __device__ __forceinline__ int wave_total_i(int v) { return __builtin_amdgcn_readlane(wave_scan_i(v), 63); }
 
+__device__ __forceinline__ int unit_seq(const Attn4Args& p, int u) {
+  return p.tiles == 1 ? u : static_cast<int>(__umulhi(static_cast<uint32_t>(u), p.tiles_inv));
+}
+
 // Keys of the unit's last live row, in [0, cap]; rows: its live rows (may be 0).
 __device__ __forceinline__ int32_t unit_keys(const Attn4Args& p, int u, int32_t& rows) {
-  const int b = p.tiles == 1 ? u : u / p.tiles, s0 = (u - b * p.tiles) * p.qt;
+  const int b = unit_seq(p, u), s0 = (u - b * p.tiles) * p.qt;
   rows = min(live_rows(p.lens, b, p.seq) - s0, p.qt);
   if (rows <= 0) return 0;
   const int64_t n = seq_position(p.start[b], s0 + rows);
@@ -97,6 +103,11 @@ __device__ __forceinline__ int unit_steps(const Attn4Args& p, int u) {
   return u < p.units ? (unit_keys(p, u, rows) + kStep - 1) / kStep : 0;
 }
 
+// Contexts of up to kWholeSteps steps are one piece, others are cut into pieces of at least
+// kMinSteps.
+constexpr int kWholeSteps = 32;
+constexpr int kMinSteps = 16;
+
 // Which unit and piece the slot takes.  per: steps of a piece.  unit < 0: no work.
 struct Piece {
   int unit, piece, pieces, first, per;  // first: slot of the unit's first piece
@@ -105,37 +116,52 @@ __device__ __forceinline__ Piece kv4_plan(const Attn4Args& p, int slot, int lane
   if (p.slots == 0) return {slot, 0, 1, slot, 1 << 26};
   // steps of a lane's units lane, lane + 64, ...: the first ones stay in a register
   const int st0 = unit_steps(p, lane);
+  if (p.units == 1) {  // nothing to share out
+    const uint32_t st = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(st0));
+    const uint32_t per = st <= kWholeSteps ? kWholeSteps
+                                           : max((st + p.slots - 1) / static_cast<uint32_t>(p.slots), static_cast<uint32_t>(p.min_steps));
+    const int n = static_cast<int>(max((st + per - 1) / per, 1u));
+    return {slot < n ? 0 : -1, slot, n, 0, static_cast<int>(per)};
+  }
   int total = wave_total_i(st0);
   for (int c = 64; c < p.units; c += 64) total += wave_total_i(unit_steps(p, c + lane));
+  // pieces of a unit of st steps: few steps stay whole (a merge costs more than they do)
+  auto split = [&](int st, int per, int u) -> int {
+    if (u >= p.units) return 0;
+    return st <= kWholeSteps ? 1 : static_cast<int>((static_cast<uint32_t>(st) + per - 1) / static_cast<uint32_t>(per));
+  };
   auto pieces_at = [&](int per) {
-    const uint32_t d = static_cast<uint32_t>(per);
-    int n = wave_total_i(lane < p.units ? max((st0 + d - 1) / d, 1u) : 0);
-    for (int c = 64; c < p.units; c += 64)
-      n += wave_total_i(c + lane < p.units ? max((unit_steps(p, c + lane) + d - 1) / d, 1u) : 0);
+    int n = wave_total_i(split(st0, per, lane));
+    for (int c = 64; c < p.units; c += 64) n += wave_total_i(split(unit_steps(p, c + lane), per, c + lane));
     return n;
   };
   // ceil(steps / per) summed over the units is at most total / per + units, so `hi` fits
   int lo = max((total + p.slots - 1) / p.slots, p.min_steps);
   int hi = max((total + p.slots - p.units - 1) / (p.slots - p.units), lo);
-  while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
+  for (int mid = lo; lo < hi; mid = (lo + hi) >> 1) {  // (equal contexts mostly fit at the first try)
     if (pieces_at(mid) <= p.slots) hi = mid;
     else lo = mid + 1;
   }
-  const uint32_t per = static_cast<uint32_t>(hi);
   int at = slot;
   for (int c = 0; c < p.units; c += 64) {
     const int st = c == 0 ? st0 : unit_steps(p, c + lane);
-    const int n = c + lane < p.units ? static_cast<int>(max((st + per - 1) / per, 1u)) : 0;
+    const int n = split(st, hi, c + lane);
     const int upto = wave_scan_i(n), all = __builtin_amdgcn_readlane(upto, 63);
     if (at < all) {
       const int i = __builtin_popcountll(__builtin_amdgcn_ballot_w64(upto <= at));
       const int mine = __builtin_amdgcn_readlane(n, i), before = __builtin_amdgcn_readlane(upto, i) - mine;
-      return {c + i, at - before, mine, slot - (at - before), hi};
+      return {c + i, at - before, mine, slot - (at - before), mine == 1 ? kWholeSteps + hi : hi};
     }
     at -= all;
   }
   return {-1, 0, 1, 0, 1};
+}
+
+// A block barrier for LDS alone: global loads that nobody needs any more stay in flight.
+__device__ __forceinline__ void lds_barrier() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
 // Parts of an fp32 value as bf16, largest first: 8 bits each.
@@ -148,8 +174,9 @@ __device__ __forceinline__ void bf16_parts(float v, __bf16 (&out)[N]) {
   }
 }
 
+// Two 8-wave blocks fit a CU (fp32 q: one): 128 registers a wave.
 template <int D, bool F32, int NW>
-__global__ __launch_bounds__(NW * 64) void kv4_attention_kernel(Attn4Args p) {
+__global__ __launch_bounds__(NW * 64, F32 ? 2 : 4) void kv4_attention_kernel(Attn4Args p) {
   constexpr int KK = D / 32;            // MFMA k steps of a score tile
   constexpr int CW = D / 16;            // dimensions per lane of a V row = output tiles
   constexpr int GR = D / 32;            // scale groups of a row
@@ -162,12 +189,12 @@ __global__ __launch_bounds__(NW * 64) void kv4_attention_kernel(Attn4Args p) {
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
   const int j = lane & 15, h = lane >> 4;
-  const int g = blockIdx.x % p.hkv;
-  const Piece at = kv4_plan(p, static_cast<int>(blockIdx.x) / p.hkv, lane);
+  const int g = blockIdx.x;
+  const Piece at = kv4_plan(p, static_cast<int>(blockIdx.y), lane);
   if (at.unit < 0) return;
   const int unit = __builtin_amdgcn_readfirstlane(at.unit), piece = __builtin_amdgcn_readfirstlane(at.piece);
   const int pieces = __builtin_amdgcn_readfirstlane(at.pieces);
-  const int b = unit / p.tiles, s0 = (unit - b * p.tiles) * p.qt;
+  const int b = unit_seq(p, unit), s0 = (unit - b * p.tiles) * p.qt;
   int32_t rows;
   const int32_t n_keys = unit_keys(p, unit, rows);
   if (rows <= 0) return;  // (a unit without live rows has one piece)
@@ -177,11 +204,13 @@ __global__ __launch_bounds__(NW * 64) void kv4_attention_kernel(Attn4Args p) {
   const int my = hi - lo > wave ? (hi - lo - wave + NW - 1) / NW : 0;  // this wave's steps
 
   // column j: position s0 + j / G, head g G + j % G; columns past the last repeat column 0
-  const int col = j < cols ? j : 0;
-  const int qrow = b * p.seq + s0 + col / p.G;
-  const int64_t qoff = (static_cast<int64_t>(qrow) * p.hq + g * p.G + col % p.G) * D + (D / 4) * h;
+  const int col = j < cols ? j : 0, crow = (col * p.g_inv) >> 16;
+  const int64_t qoff = (static_cast<int64_t>(b * p.seq + s0 + crow) * p.hq + g * p.G + col - crow * p.G) * D + (D / 4) * h;
   const int32_t limit = static_cast<int32_t>(
-      min(max(seq_position(p.start[b], s0 + col / p.G + 1), int64_t{0}), static_cast<int64_t>(p.cap)));  // keys of the column
+      min(max(seq_position(p.start[b], s0 + crow + 1), int64_t{0}), static_cast<int64_t>(p.cap)));  // keys of the column
+  // the first column's: steps up to it need no mask
+  const int32_t least = static_cast<int32_t>(
+      min(max(seq_position(p.start[b], s0 + 1), int64_t{0}), static_cast<int64_t>(p.cap)));
   bf16x8_t qop[QP][KK];
 #pragma unroll
   for (int kk = 0; kk < KK; ++kk) {
@@ -201,29 +230,35 @@ __global__ __launch_bounds__(NW * 64) void kv4_attention_kernel(Attn4Args p) {
     }
   }
 
-  struct Buf {
-    uint32_t k[2][KK];   // codes of the lane's D/4 dimensions of two keys
-    uint32_t ks[2];      // their scale bytes
-    uint32_t v[8];       // CW codes of 8 keys
-    uint32_t vs[2][GR];  // all scale bytes of two runs of 4 keys
-  };
-  auto issue = [&](Buf& bf, int i) {
-    const int64_t off = p.kv.Row(b, g, static_cast<int64_t>(kStep) * (lo + wave + i * NW));
+  // One step's codes and scale bytes in registers.  K of the next step is loaded once this
+  // step's scores are taken, V once its products are, so one of the two is always in flight
+  // behind the other's work.  (A load past the wave's last step reads that step again: a branch
+  // around it would make every wait count on the worse of its two sides.)
+  uint32_t k_code[2][KK];   // the lane's D/4 dimensions of two keys
+  uint32_t k_scale[2];      // their scale bytes
+  uint32_t v_code[8];       // CW codes of 8 keys
+  uint32_t v_scale[2][GR];  // all scale bytes of two runs of 4 keys
+  auto step_rows = [&](int i) { return p.kv.Row(b, g, static_cast<int64_t>(kStep) * (lo + wave + min(i, my - 1) * NW)); };
+  auto issue_k = [&](int64_t off) {
     const uint8_t* kc = p.kc + off / 2;
-    const uint8_t* vc = p.vc + off / 2;
     const uint8_t* ks = p.ks + off / 32;
-    const uint8_t* vs = p.vs + off / 32;
 #pragma unroll
     for (int tt = 0; tt < 2; ++tt) {
-      __builtin_memcpy(bf.k[tt], __builtin_assume_aligned(kc + (16 * tt + j) * (D / 2) + (D / 8) * h, D / 8), D / 8);
-      bf.ks[tt] = ks[(16 * tt + j) * GR + h * GR / 4];
-      __builtin_memcpy(bf.vs[tt], __builtin_assume_aligned(vs + (16 * tt + 4 * h) * GR, 4 * GR), 4 * GR);
+      __builtin_memcpy(k_code[tt], __builtin_assume_aligned(kc + (16 * tt + j) * (D / 2) + (D / 8) * h, D / 8), D / 8);
+      k_scale[tt] = ks[(16 * tt + j) * GR + h * GR / 4];
     }
+  };
+  auto issue_v = [&](int64_t off) {
+    const uint8_t* vc = p.vc + off / 2;
+    const uint8_t* vs = p.vs + off / 32;
+#pragma unroll
+    for (int tt = 0; tt < 2; ++tt)
+      __builtin_memcpy(v_scale[tt], __builtin_assume_aligned(vs + (16 * tt + 4 * h) * GR, 4 * GR), 4 * GR);
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const uint8_t* at_v = vc + (16 * (e >> 2) + 4 * h + (e & 3)) * (D / 2) + (CW / 2) * j;
-      if constexpr (CW == 8) bf.v[e] = *reinterpret_cast<const uint32_t*>(at_v);
-      else bf.v[e] = *reinterpret_cast<const uint16_t*>(at_v);
+      if constexpr (CW == 8) v_code[e] = *reinterpret_cast<const uint32_t*>(at_v);
+      else v_code[e] = *reinterpret_cast<const uint16_t*>(at_v);
     }
   };
 
@@ -233,23 +268,38 @@ __global__ __launch_bounds__(NW * 64) void kv4_attention_kernel(Attn4Args p) {
 #pragma unroll
   for (int t = 0; t < CW; ++t) o[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 
-  auto compute = [&](const Buf& bf, int i) {
-    const int32_t base = kStep * (lo + wave + i * NW) + 4 * h;  // key of score (0, 0)
+  if (my > 0) {
+    const int64_t off = step_rows(0);
+    issue_k(off);
+    issue_v(off);
+  }
+  for (int i = 0; i < my; ++i) {
+    const int64_t next = step_rows(i + 1);
+    const int32_t first = kStep * (lo + wave + i * NW);  // key of the step
+    const int32_t base = first + 4 * h;                  // of this lane's score (0, 0)
     float sc[8];
 #pragma unroll
     for (int tt = 0; tt < 2; ++tt) {
       f32x4_t acc = f32x4_t{0.f, 0.f, 0.f, 0.f};
-      const float s = e8m0_scale_or_nan(bf.ks[tt]);
+      const float s = e8m0_scale_or_nan(k_scale[tt]);
 #pragma unroll
       for (int kk = 0; kk < KK; ++kk) {
         uint32_t w[4];
-        fp4_to_bf16(bf.k[tt][kk], s, w);
+        fp4_to_bf16(k_code[tt][kk], s, w);
         const bf16x8_t a = __builtin_bit_cast(bf16x8_t, make_uint4(w[0], w[1], w[2], w[3]));
 #pragma unroll
         for (int i2 = QP - 1; i2 >= 0; --i2) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, qop[i2][kk], acc, 0, 0, 0);
       }
 #pragma unroll
-      for (int r = 0; r < 4; ++r) sc[4 * tt + r] = base + 16 * tt + r < limit ? acc[r] : -INFINITY;
+      for (int r = 0; r < 4; ++r) sc[4 * tt + r] = acc[r];
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    issue_k(next);
+    __builtin_amdgcn_sched_barrier(0);
+    if (first + kStep > least) {  // (wave-uniform) some column ends in this step
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (base + 16 * (e >> 2) + (e & 3) >= limit) sc[e] = -INFINITY;
     }
     float bm = sc[0];
 #pragma unroll
@@ -270,16 +320,21 @@ __global__ __launch_bounds__(NW * 64) void kv4_attention_kernel(Attn4Args p) {
     }
     // (a column without a live key subtracts 0: exp2(-inf) is 0)
     const float sub = m_run == -INFINITY ? 0.0f : -m_run;
-    bf16x8_t pop[PP];
+    uint32_t pw[PP][4];
     float sum = 0.0f;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float v = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[e], p.scale, sub));
-      sum += v;
-      __bf16 t[PP];
-      bf16_parts<PP>(v, t);
+    for (int e = 0; e < 8; e += 2) {
+      float v0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[e], p.scale, sub));
+      float v1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[e + 1], p.scale, sub));
+      sum += v0;
+      sum += v1;
 #pragma unroll
-      for (int i2 = 0; i2 < PP; ++i2) pop[i2][e] = t[i2];
+      for (int i2 = 0; i2 < PP; ++i2) {
+        const uint32_t w = __builtin_bit_cast(uint32_t, bf16x2_t{static_cast<__bf16>(v0), static_cast<__bf16>(v1)});
+        pw[i2][e / 2] = w;
+        v0 -= __uint_as_float(w << 16);
+        v1 -= __uint_as_float(w & 0xFFFF0000u);
+      }
     }
     l_run += sum;
     // V: a NaN value must not reach the product, where the probability 0 of a key behind some
@@ -288,8 +343,8 @@ __global__ __launch_bounds__(NW * 64) void kv4_attention_kernel(Attn4Args p) {
     uint32_t sb[8], most = 0;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      if constexpr (GR == 4) sb[e] = (bf.vs[e >> 2][e & 3] >> (8 * (j >> 2))) & 0xFFu;
-      else sb[e] = (bf.vs[e >> 2][(e & 3) >> 1] >> (16 * (e & 1) + 8 * (j >> 3))) & 0xFFu;
+      if constexpr (GR == 4) sb[e] = (v_scale[e >> 2][e & 3] >> (8 * (j >> 2))) & 0xFFu;
+      else sb[e] = (v_scale[e >> 2][(e & 3) >> 1] >> (16 * (e & 1) + 8 * (j >> 3))) & 0xFFu;
       most = max(most, sb[e]);
     }
     if (__builtin_amdgcn_ballot_w64(most >= kScaleNan) != 0) {
@@ -302,41 +357,34 @@ __global__ __launch_bounds__(NW * 64) void kv4_attention_kernel(Attn4Args p) {
         }
       }
     }
-    uint32_t pr[8][CW / 2];
+    // two neighbouring dimensions (output tiles 2 t2, 2 t2 + 1) of the lane's 8 keys at a time
+    auto tile_pair = [&]<int T2>() {
+      uint32_t pr[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float s = e8m0_scale(sb[e]);
-      pr[e][0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(bf.v[e], s, 0));
-      pr[e][1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(bf.v[e], s, 1));
-      if constexpr (CW == 8) {
-        pr[e][2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(bf.v[e], s, 2));
-        pr[e][3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(bf.v[e], s, 3));
+      for (int e = 0; e < 8; ++e)
+        pr[e] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(v_code[e], e8m0_scale(sb[e]), T2));
+#pragma unroll
+      for (int odd = 0; odd < 2; ++odd) {
+        uint32_t w[4];
+#pragma unroll
+        for (int e2 = 0; e2 < 4; ++e2)
+          w[e2] = __builtin_amdgcn_perm(pr[2 * e2 + 1], pr[2 * e2], odd ? 0x07060302u : 0x05040100u);
+        const bf16x8_t vop = __builtin_bit_cast(bf16x8_t, make_uint4(w[0], w[1], w[2], w[3]));
+#pragma unroll
+        for (int i2 = PP - 1; i2 >= 0; --i2)
+          o[2 * T2 + odd] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+              __builtin_bit_cast(bf16x8_t, make_uint4(pw[i2][0], pw[i2][1], pw[i2][2], pw[i2][3])), vop, o[2 * T2 + odd], 0, 0, 0);
       }
+    };
+    tile_pair.template operator()<0>();
+    tile_pair.template operator()<1>();
+    if constexpr (CW == 8) {
+      tile_pair.template operator()<2>();
+      tile_pair.template operator()<3>();
     }
-#pragma unroll
-    for (int t = 0; t < CW; ++t) {
-      uint32_t w[4];
-#pragma unroll
-      for (int e2 = 0; e2 < 4; ++e2) {
-        const uint32_t a0 = pr[2 * e2][t >> 1], a1 = pr[2 * e2 + 1][t >> 1];
-        w[e2] = (t & 1) ? ((a0 >> 16) | (a1 & 0xFFFF0000u)) : ((a0 & 0xFFFFu) | (a1 << 16));
-      }
-      const bf16x8_t vop = __builtin_bit_cast(bf16x8_t, make_uint4(w[0], w[1], w[2], w[3]));
-#pragma unroll
-      for (int i2 = PP - 1; i2 >= 0; --i2) o[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pop[i2], vop, o[t], 0, 0, 0);
-    }
-  };
-
-  if (my > 0) {
-    Buf ba, bb;
-    issue(ba, 0);
-    for (int i = 0; i < my; i += 2) {
-      if (i + 1 < my) issue(bb, i + 1);
-      compute(ba, i);
-      if (i + 1 >= my) break;
-      if (i + 2 < my) issue(ba, i + 2);
-      compute(bb, i + 1);
-    }
+    __builtin_amdgcn_sched_barrier(0);
+    issue_v(next);
+    __builtin_amdgcn_sched_barrier(0);
   }
 
   // NaN values: the columns that have the key, in its group's dimensions
@@ -368,61 +416,69 @@ __global__ __launch_bounds__(NW * 64) void kv4_attention_kernel(Attn4Args p) {
       for (int t = 0; t < CW; ++t) so[c * D + CW * j + t] = o[t][r];
     }
   }
-  __syncthreads();
-  const float* sm0 = smem + static_cast<int64_t>(NW) * ncol * D;
-  // merge of the waves for 4 dimensions of a column
-  auto wave_merge = [&](int c, int d0, float& mx, float& den, f32x4_t& acc) {
-    mx = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < NW; ++w) mx = fmaxf(mx, sm0[w * 32 + c]);
-    den = 0.0f;
-    acc = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    // (a NaN score leaves the maximum and makes its wave's sum NaN)
+  lds_barrier();
+  // From here on every instruction runs once per block, so the fetch of the code itself costs
+  // more than its work: loops stay rolled where their latency allows it.
+  const int items = cols * (D / 4);  // 4 dimensions of a column
+  const float* sm0 = smem + NW * ncol * D;
+  auto wave_merge = [&](int t, float& mx, float& den, f32x4_t& acc) {
+    const int c = t / (D / 4);
+    float m[NW], l[NW];
+    f32x4_t v[NW];
 #pragma unroll
     for (int w = 0; w < NW; ++w) {
-      const float m = sm0[w * 32 + c], f = mx == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mx);
-      den = __builtin_fmaf(sm0[w * 32 + 16 + c], f, den);
-      const f32x4_t v = *reinterpret_cast<const f32x4_t*>(smem + (static_cast<int64_t>(w) * ncol + c) * D + d0);
+      m[w] = sm0[w * 32 + c];
+      l[w] = sm0[w * 32 + 16 + c];
+      v[w] = *reinterpret_cast<const f32x4_t*>(smem + w * ncol * D + 4 * t);
+    }
+    mx = m[0];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) acc[e] = __builtin_fmaf(v[e], f, acc[e]);
-    }
-  };
-  auto write_out = [&](int c, int d0, float den, const f32x4_t& acc) {
-    const int64_t to = (static_cast<int64_t>(b * p.seq + s0 + c / p.G) * p.hq + g * p.G + c % p.G) * D + d0;
+    for (int w = 1; w < NW; ++w) mx = fmaxf(mx, m[w]);
+    // (a NaN score leaves the maximum and makes its wave's sum NaN)
+    const float top = mx == -INFINITY ? 0.0f : mx;
+    den = 0.0f;
+    acc = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float v = den == 0.0f ? 0.0f : acc[e] / den;  // no keys: zeros; a NaN sum stays
-      if constexpr (F32) static_cast<float*>(p.out)[to + e] = v;
-      else static_cast<uint16_t*>(p.out)[to + e] = f32_to_bf16_bits(v);
+    for (int w = 0; w < NW; ++w) {
+      const float f = __builtin_amdgcn_exp2f(m[w] - top);
+      den = __builtin_fmaf(l[w], f, den);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[e] = __builtin_fmaf(v[w][e], f, acc[e]);
     }
   };
-  if (pieces == 1) {
-    for (int t = threadIdx.x; t < cols * (D / 4); t += NT) {
-      const int c = t / (D / 4), d0 = 4 * (t % (D / 4));
-      float mx, den;
-      f32x4_t acc;
-      wave_merge(c, d0, mx, den, acc);
-      write_out(c, d0, den, acc);
+  auto write_out = [&](int t, float den, const f32x4_t& acc) {
+    const int c = t / (D / 4), d0 = 4 * (t % (D / 4)), row = (c * p.g_inv) >> 16;
+    const int64_t to = (static_cast<int64_t>(b * p.seq + s0 + row) * p.hq + g * p.G + c - row * p.G) * D + d0;
+    const float inv = den == 0.0f ? 0.0f : 1.0f / den;  // no keys: zeros; a NaN sum stays
+    f32x4_t v;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = acc[e] * inv;
+    if constexpr (F32) {
+      *reinterpret_cast<f32x4_t*>(static_cast<float*>(p.out) + to) = v;
+    } else {
+      const uint32_t w0 = f32_to_bf16_bits(v[0]) | (static_cast<uint32_t>(f32_to_bf16_bits(v[1])) << 16);
+      const uint32_t w1 = f32_to_bf16_bits(v[2]) | (static_cast<uint32_t>(f32_to_bf16_bits(v[3])) << 16);
+      *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + to) = make_uint2(w0, w1);
     }
-    return;
-  }
-  const int rec_floats = ncol * RH;
-  auto record = [&](int pc) {
-    float* r = p.part + (static_cast<int64_t>(at.first + pc) * p.hkv + g) * rec_floats;
-    return __builtin_amdgcn_make_buffer_rsrc(r, 0, rec_floats * 4, kRawBufferFlags);
   };
-  {
-    const __amdgpu_buffer_rsrc_t mine = record(piece);
-    for (int t = threadIdx.x; t < cols * (D / 4); t += NT) {
-      const int c = t / (D / 4), d0 = 4 * (t % (D / 4));
-      float mx, den;
-      f32x4_t acc;
-      wave_merge(c, d0, mx, den, acc);
-      if (d0 == 0)
-        __builtin_amdgcn_raw_buffer_store_b64(u32x2_t{__float_as_uint(mx), __float_as_uint(den)}, mine, c * RH * 4, 0, kCpolSc1);
-      __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4_t, acc), mine, (c * RH + 4 + d0) * 4, 0, kCpolSc1);
+  // the unit's records: piece_bytes apart (at most kMaxSlotHeads records in all: 35 MB)
+  const int piece_bytes = p.hkv * ncol * RH * 4;
+  const __amdgpu_buffer_rsrc_t all = __builtin_amdgcn_make_buffer_rsrc(
+      p.part + (static_cast<int64_t>(at.first) * p.hkv + g) * (ncol * RH), 0, (pieces - 1) * piece_bytes + ncol * RH * 4, kRawBufferFlags);
+  for (int t = threadIdx.x; t < items; t += NT) {
+    float mx, den;
+    f32x4_t acc;
+    wave_merge(t, mx, den, acc);
+    if (pieces == 1) {
+      write_out(t, den, acc);
+    } else {
+      const int c = t / (D / 4), at_rec = piece * piece_bytes + c * RH * 4;
+      if (t % (D / 4) == 0)
+        __builtin_amdgcn_raw_buffer_store_b64(u32x2_t{__float_as_uint(mx), __float_as_uint(den)}, all, at_rec, 0, kCpolSc1);
+      __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4_t, acc), all, at_rec + 16 + 16 * (t % (D / 4)), 0, kCpolSc1);
     }
   }
+  if (pieces == 1) return;
   __builtin_amdgcn_s_waitcnt(0);  // acknowledged before the ticket
   __syncthreads();
   unsigned* ticket = p.tickets + at.first * p.hkv + g;
@@ -430,49 +486,79 @@ __global__ __launch_bounds__(NW * 64) void kv4_attention_kernel(Attn4Args p) {
     last = __hip_atomic_fetch_add(ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == static_cast<unsigned>(pieces - 1);
   __syncthreads();
   if (!last) return;
-  // Merge in piece order, kBatch records in flight at a time.
-  constexpr int kBatch = 8;
-  for (int t = threadIdx.x; t < cols * (D / 4); t += NT) {
-    const int c = t / (D / 4), d0 = 4 * (t % (D / 4));
+  // Merge: the threads form teams of one thread per 4 dimensions of a column; team w takes
+  // the pieces w, w + teams, ..., kBatch records in flight at a time, and the teams' sums meet
+  // in LDS (NW / 2 teams fit where the waves' states were).  The order follows from the shape
+  // alone.
+  constexpr int kBatch = 4;
+  const int teams = max(1, min(NT / items, NW / 2)), team = teams == 1 ? 0 : static_cast<int>(threadIdx.x) / items;
+  float* state = smem;  // (the waves' states are consumed) per team and item: m, l, 2 pad, o[4]
+  for (int t = threadIdx.x - team * items; t < items && team < teams; t += NT) {
+    const int c = t / (D / 4);
     float mx = -INFINITY, den = 0.0f;
     f32x4_t acc = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    for (int r0 = 0; r0 < pieces; r0 += kBatch) {
+    int off = team * piece_bytes + c * RH * 4;  // (reads past the last record give zeros)
+#pragma unroll 1
+    for (int r0 = team; r0 < pieces; r0 += kBatch * teams) {
       u32x2_t ml[kBatch];
       u32x4_t ov[kBatch];
 #pragma unroll
       for (int u = 0; u < kBatch; ++u) {
-        const __amdgpu_buffer_rsrc_t rec = record(min(r0 + u, pieces - 1));
-        ml[u] = __builtin_amdgcn_raw_buffer_load_b64(rec, c * RH * 4, 0, kCpolSc1);
-        ov[u] = __builtin_amdgcn_raw_buffer_load_b128(rec, (c * RH + 4 + d0) * 4, 0, kCpolSc1);
+        ml[u] = __builtin_amdgcn_raw_buffer_load_b64(all, off, 0, kCpolSc1);
+        ov[u] = __builtin_amdgcn_raw_buffer_load_b128(all, off + 16 + 16 * (t % (D / 4)), 0, kCpolSc1);
+        off += teams * piece_bytes;
       }
-      float bm = mx;
+      float bm = mx, m[kBatch];
 #pragma unroll
-      for (int u = 0; u < kBatch; ++u) bm = fmaxf(bm, __uint_as_float(ml[u][0]));
-      const float f0 = bm == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(mx - bm);
+      for (int u = 0; u < kBatch; ++u) {
+        m[u] = r0 + u * teams < pieces ? __uint_as_float(ml[u][0]) : -INFINITY;
+        bm = fmaxf(bm, m[u]);
+      }
+      const float top = bm == -INFINITY ? 0.0f : bm;  // (then every l and o is 0 or NaN, and its factor 0: NaN stays)
+      const float f0 = __builtin_amdgcn_exp2f(mx - top);
       den *= f0;
 #pragma unroll
       for (int e = 0; e < 4; ++e) acc[e] *= f0;
 #pragma unroll
       for (int u = 0; u < kBatch; ++u) {
-        if (r0 + u >= pieces) break;
-        const float f = bm == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(__uint_as_float(ml[u][0]) - bm);
+        const float f = __builtin_amdgcn_exp2f(m[u] - top);
         den = __builtin_fmaf(__uint_as_float(ml[u][1]), f, den);
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc[e] = __builtin_fmaf(__uint_as_float(ov[u][e]), f, acc[e]);
       }
       mx = bm;
     }
-    write_out(c, d0, den, acc);
+    float* st = state + (team * items + t) * 8;
+    *reinterpret_cast<f32x4_t*>(st) = f32x4_t{mx, den, 0.f, 0.f};
+    *reinterpret_cast<f32x4_t*>(st + 4) = acc;
+  }
+  __syncthreads();
+  for (int t = threadIdx.x; t < items; t += NT) {
+    float mx = -INFINITY, den = 0.0f;
+    f32x4_t acc = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+    for (int w = 0; w < teams; ++w) mx = fmaxf(mx, state[(w * items + t) * 8]);
+    mx = mx == -INFINITY ? 0.0f : mx;
+#pragma unroll 1
+    for (int w = 0; w < teams; ++w) {
+      const float* st = state + (w * items + t) * 8;
+      const float f = __builtin_amdgcn_exp2f(st[0] - mx);
+      den = __builtin_fmaf(st[1], f, den);
+      const f32x4_t v = *reinterpret_cast<const f32x4_t*>(st + 4);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[e] = __builtin_fmaf(v[e], f, acc[e]);
+    }
+    write_out(t, den, acc);
   }
   if (threadIdx.x == 0) __hip_atomic_store(ticket, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
-constexpr int kWaves = 4;
-constexpr int kMinSteps = 4;  // fewest steps of a piece
+constexpr int kWaves = 8;
+constexpr int64_t kMaxRows = 65535;  // query rows of a call
 
 // Slots of the planned grid (0: a block per unit and kv head without a plan).
 int64_t Slots(int64_t units, int64_t hkv, int64_t capacity) {
-  const int64_t target = 2 * DeviceCUs();
+  const int64_t cus = DeviceCUs(), target = 4 * units * hkv < cus ? cus : 2 * cus;
   if (units * hkv >= target || units * CeilDiv(capacity, kStep) >= (int64_t{1} << 30)) return 0;
   const int64_t slots = std::max(CeilDiv(target, hkv), 2 * units);
   return slots * hkv <= kMaxSlotHeads ? slots : 0;
@@ -484,10 +570,12 @@ int64_t WorkspaceBytes(int64_t units, int64_t qt, int64_t G, int64_t hkv, int64_
 
 template <int D, bool F32>
 void Launch(const Attn4Args& p, hipStream_t s) {
-  const int64_t grid = static_cast<int64_t>(p.slots > 0 ? p.slots : p.units) * p.hkv;
-  const int lds = kWaves * (p.qt * p.G * D + 32) * 4;
-  RecordLaunch(grid, kWaves * 64, lds, "kv4_attention<%s,d=%d,waves=%d,slots=%d>", F32 ? "f32" : "bf16", D, kWaves, p.slots);
-  hipLaunchKernelGGL((kv4_attention_kernel<D, F32, kWaves>), dim3(static_cast<unsigned>(grid)), dim3(kWaves * 64), lds, s, p);
+  // kv head fastest: with 8 kv heads every block of a head runs on one XCD
+  const dim3 grid(static_cast<unsigned>(p.hkv), static_cast<unsigned>(p.slots > 0 ? p.slots : p.units));
+  constexpr int NW = kWaves;
+  const int lds = NW * (p.qt * p.G * D + 32) * 4;
+  RecordLaunch(static_cast<int64_t>(grid.x) * grid.y, NW * 64, lds, "kv4_attention<%s,d=%d,waves=%d,slots=%d>", F32 ? "f32" : "bf16", D, NW, p.slots);
+  hipLaunchKernelGGL((kv4_attention_kernel<D, F32, NW>), grid, dim3(NW * 64), lds, s, p);
 }
 
 }  // namespace
@@ -508,8 +596,8 @@ extern "C" am_status_code am_gfx950_kv4_attention(const am_gfx950_kv4_attention_
   AM_CHECK_ARG(a->hq > 0 && a->hkv > 0 && a->hq % a->hkv == 0, "kv4_attention: q heads must be a multiple of kv heads");
   AM_CHECK_ARG(a->hq / a->hkv <= 16, "kv4_attention: at most 16 q heads per kv head");
   AM_CHECK_ARG(a->batch >= 0 && a->seq >= 0 && a->capacity > 0 && a->capacity < (int64_t{1} << 31) - 64, "kv4_attention: bad shape");
-  AM_CHECK_ARG(a->batch <= 65535 && a->seq <= (1 << 24) && a->hkv <= 65536 && a->batch * a->seq <= (1 << 24) &&
-                   a->batch * a->seq * a->hkv <= (1 << 24), "kv4_attention: too many query rows");
+  AM_CHECK_ARG(a->hkv <= 65536 && a->batch <= kMaxRows && a->seq <= kMaxRows && a->batch * a->seq <= kMaxRows,
+               "kv4_attention: too many query rows");
   AM_CHECK_ARG(std::isfinite(a->scale) && a->scale >= 0.0f, "kv4_attention: scale must be finite and not negative");
   if (a->batch == 0 || a->seq == 0) return AM_STATUS_OK;
   AM_CHECK_ARG(a->q && a->out && a->start_pos_dev, "kv4_attention: null pointer");
@@ -536,6 +624,8 @@ extern "C" am_status_code am_gfx950_kv4_attention(const am_gfx950_kv4_attention_
   p.cap = static_cast<int32_t>(a->capacity);
   p.slots = static_cast<int32_t>(Slots(units, a->hkv, a->capacity));
   p.min_steps = kMinSteps;
+  p.tiles_inv = static_cast<uint32_t>(CeilDiv(int64_t{1} << 32, tiles));
+  p.g_inv = static_cast<int32_t>(CeilDiv(1 << 16, G));
   p.scale = kLog2e * (a->scale > 0.0f ? a->scale : 1.0f / sqrtf(static_cast<float>(a->head_dim)));
   hipStream_t s = AsStream(stream);
   if (a->dtype == AM_DT_BF16) a->head_dim == 128 ? Launch<128, false>(p, s) : Launch<64, false>(p, s);

@@ -409,8 +409,8 @@ am_status_code am_gfx950_kv4_read(const am_gfx950_kv4_read_args* args, void* hip
  * positions up to it, below capacity: a row before position 0 has no keys and gives zeros,
  * one past the cache has all of them.  Rows behind seq_lens[b] are left as they were.
  * out = sum_t softmax_t(scale * q . K_t) V_t over the values that the cache stands for;
- * q head h reads kv head h / (hq / hkv), at most 16 q heads per kv head; fp32 online
- * softmax; the products take q as it is (bf16) or as three bf16 parts (fp32) and the
+ * q head h reads kv head h / (hq / hkv), at most 16 q heads per kv head and 65535 query
+ * rows; fp32 online softmax; the products take q as it is (bf16) or as three bf16 parts (fp32) and the
  * probabilities as two or three, so neither adds to the one rounding of out.  Scores of
  * which none exceeds minus infinity give zeros.  A NaN among a row's keys gives NaN (a NaN
  * value only in its own 32 dimensions); what the cache holds past a row's keys does not
