@@ -47,7 +47,7 @@ struct Attn4Args {
   int32_t slots;  // planned grid; 0: one piece per unit
   int32_t min_steps;
   uint32_t tiles_inv;  // ceil(2^32 / tiles): unit / tiles by a multiplication (below 2^16 units)
-  int32_t g_inv;  // ceil(2^16 / G): c / G = (c * g_inv) >> 16 for a column c < 16
+  int32_t g_inv;  // ceil(2^16 / G): c / G = (c * g_inv) >> 16 for a column c < 32
   float scale;  // of the scores, times log2(e)
 };
 
@@ -553,6 +553,524 @@ __global__ __launch_bounds__(NW * 64, F32 ? 2 : 4) void kv4_attention_kernel(Att
   if (threadIdx.x == 0) __hip_atomic_store(ticket, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
+// ---- many query rows ----
+//
+// A block owns 4 x 32 MFMA columns (32 / G query positions with their G heads per wave) of one
+// kv head and walks the keys up to its last row's in tiles of 32, in two key groups of four
+// waves that take every other tile and merge in LDS:
+//   * A group's threads load the codes of a tile two intervals ahead, and convert them into one
+//     of four LDS buffers, K and V row-major with their 16-byte slots XORed by the key, so that
+//     the operand reads meet no bank twice.  A conversion serves all the group's columns.
+//   * S^T = K Q^T on v_mfma_f32_32x32x16_bf16: lane (j, h) holds column j's scores of keys
+//     8 (r >> 2) + 4 h + (r & 3), and these are the k slots of its P operand in
+//     O^T = V^T P^T: P stays in its lane, and so does the softmax state of column j, whose
+//     rescaling needs no exchange.  V^T's operand comes from the row-major tile through
+//     ds_read_b64_tr_b16.
+//   * bf16 q: P is f16, 11 bits where bf16 has 8 (its rounding is 1/8 of out's own), in one
+//     product instead of the two of a bf16 split.  V is f16 as well: codes times 2^(e - E) with E
+//     the largest scale of the group's 32 dimensions among the block's keys, less 13, and exact
+//     to 2^-36 of that largest one; the block reads its keys' scale bytes once beforehand (1/17 of
+//     the cache).  P carries 2^14 so that its small values stay normal.  Row sums are those of
+//     the rounded P.  fp32 q: three bf16 parts of q and P, bf16 V.
+//   * The same pass over the scales finds the first NaN value of each group; it enters the
+//     products as zero and spoils the columns that see its key at the end.
+// What bounds it: VALU work (a tile costs a wave about 120 instructions, 57 of them the
+// softmax's, beside 16 MFMAs), which the MFMAs of the SIMD's other wave hide.
+typedef __attribute__((ext_vector_type(8))) _Float16 f16x8_t;
+typedef __attribute__((ext_vector_type(2))) _Float16 f16x2_t;
+typedef __attribute__((ext_vector_type(16))) float f32x16_t;
+typedef __attribute__((ext_vector_type(4))) short s16x4_t;
+typedef __attribute__((ext_vector_type(2))) unsigned short u16x2_t;
+constexpr int kWideWaves = 4;   // waves of columns of a block
+constexpr int kVTop = 140;      // exponent byte of the largest scale of V in f16: 6 * 2^13
+constexpr float kPBias = 14.0f;  // log2 of the factor on P in f16
+
+__device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2_t, a), __builtin_bit_cast(u16x2_t, b)));
+}
+
+// Slot of a tile's row (D values, SL slots of 16 bytes) that holds slot s of key `key`: the 16
+// keys of an operand read of K lie in 16 different slots of the banks' 256 bytes, and so do
+// the 4 keys x 4 slots of half a transposed read of V.
+template <int SL>
+__device__ __forceinline__ int k_slot(int key, int s) {
+  return s ^ (SL == 16 ? key & 15 : (key >> 1) & 7);
+}
+template <int SL>
+__device__ __forceinline__ int v_slot(int key, int s) {
+  return s ^ (4 * (SL == 16 ? key & 3 : (key >> 1) & 1));
+}
+
+// Row offsets of the 32-key tiles of (b, g), in elements: KvRows::Row of key 32 t without a
+// load that would wait among the LDS reads.  A lane holds one of 64 block-table entries; planes
+// are one block without end.
+struct TileWalk {
+  const int32_t* table;
+  int64_t block_elems, base;
+  int32_t num_blocks, stride, tile_shift, tile_mask, loaded = -1, entry = 0, lane, tile_elems;
+
+  __device__ __forceinline__ TileWalk(const KvRows& kv, int64_t b, int64_t g, int lane_) : lane(lane_), tile_elems(kStep * kv.d) {
+    if (kv.table == nullptr) {
+      table = nullptr;
+      block_elems = 0;
+      base = kv.Row(b, g, 0);
+      tile_shift = 31;
+      tile_mask = 0x7FFFFFFF;
+      loaded = 0;
+    } else {
+      table = kv.table + b * kv.stride;
+      block_elems = (static_cast<int64_t>(kv.hkv) << kv.shift) * kv.d;
+      base = (g << kv.shift) * kv.d;
+      tile_shift = kv.shift - 5;
+      tile_mask = (1 << tile_shift) - 1;
+    }
+    num_blocks = static_cast<int32_t>(min(kv.num_blocks, int64_t{0x7FFFFFFF}));
+    stride = kv.stride;
+  }
+  __device__ __forceinline__ int64_t operator()(int t) {
+    const int blk = t >> tile_shift;
+    if ((blk >> 6) != loaded) {  // (wave-uniform)
+      loaded = blk >> 6;
+      const int32_t e = table[min((blk & ~63) + lane, stride - 1)];
+      entry = min(max(e, 0), num_blocks - 1);  // entries outside the pool are clamped into it
+    }
+    return __builtin_amdgcn_readlane(entry, blk & 63) * block_elems + base + static_cast<int64_t>(t & tile_mask) * tile_elems;
+  }
+};
+
+template <int D, bool F32>
+__global__ __launch_bounds__(512) void kv4_attention_wide_kernel(Attn4Args p) {
+  constexpr int QW = kWideWaves, KS = 2;              // waves of a key group, key groups
+  constexpr int GR = D / 32, SL = D / 8;              // scale groups and 16-byte slots of a row
+  constexpr int NT = QW * KS * 64, GT = QW * 64;      // threads of the block, of a key group
+  constexpr int PC = kStep * SL;                      // pieces (8 values) of a tile of K, of V
+  constexpr int NP = 2 * PC / GT;                     // pieces of a thread per tile
+  constexpr int QP = F32 ? 3 : 1;
+  constexpr int DT = D / 32;
+  constexpr int OW = DT * 16 + 2;                     // words of a lane's state
+  static_assert(PC % GT == 0 && GT % SL == 0, "a thread's pieces are K or V by their number alone");
+  constexpr int kTileBytes = kStep * D * 2;
+  constexpr int NB = 4;                               // buffers of a key group
+  constexpr int kSmem = std::max(KS * NB * 2 * kTileBytes, (KS - 1) * QW * OW * 256);
+  static_assert(NT == 512, "two waves per SIMD, one of each half");
+  __shared__ __align__(16) uint8_t smem_w[kSmem];     // per key group and buffer: K, V
+  __shared__ uint32_t s_top[GR];                      // largest scale of V
+  __shared__ int32_t s_nan[GR];                       // first key with a NaN value
+
+  const int kg = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / GT);
+  const int tid = static_cast<int>(threadIdx.x) - kg * GT, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int j = lane & 31, h = lane >> 5;
+  // kv head fastest, then the row blocks of all sequences, last (longest) first
+  const int g = blockIdx.x;
+  const int unit = p.units - 1 - static_cast<int>(blockIdx.y), b = unit_seq(p, unit);
+  const int s0 = (unit - b * p.tiles) * (QW * p.qt);
+  const int live = min(live_rows(p.lens, b, p.seq) - s0, QW * p.qt);  // live rows of the block
+  if (live <= 0) return;
+  auto keys_of = [&](int row) {  // keys of row s0 + row
+    return static_cast<int32_t>(min(max(seq_position(p.start[b], s0 + row + 1), int64_t{0}), static_cast<int64_t>(p.cap)));
+  };
+  const int32_t kend = keys_of(live - 1);
+  const int ntiles = (kend + kStep - 1) / kStep;
+
+  // column j: position s0 + wave qt + j / G, head g G + j % G; columns behind the live rows
+  // repeat the last row
+  const int wrow = wave * p.qt;
+  const int jrow = min((j * p.g_inv) >> 16, p.qt - 1), jhead = min(j - jrow * p.G, p.G - 1);
+  const int row = min(wrow + jrow, live - 1);
+  const bool mine = j < p.qt * p.G && wrow + jrow < live;
+  const int64_t qrow = (static_cast<int64_t>(b * p.seq + s0 + row) * p.hq + g * p.G + jhead) * D;
+  const int32_t limit = keys_of(row), least = keys_of(wrow);
+  bf16x8_t qop[QP][D / 16];
+#pragma unroll
+  for (int kk = 0; kk < D / 16; ++kk) {
+    if constexpr (F32) {
+      const f32x4_t* qp = reinterpret_cast<const f32x4_t*>(static_cast<const float*>(p.q) + qrow + 16 * kk + 8 * h);
+      const f32x4_t x[2] = {qp[0], qp[1]};
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        __bf16 t[QP];
+        bf16_parts<QP>(x[e >> 2][e & 3], t);
+#pragma unroll
+        for (int i = 0; i < QP; ++i) qop[i][kk][e] = t[i];
+      }
+    } else {
+      qop[0][kk] = *reinterpret_cast<const bf16x8_t*>(static_cast<const uint16_t*>(p.q) + qrow + 16 * kk + 8 * h);
+    }
+  }
+
+  if constexpr (F32) {  // (the parts stay in registers: the compiler would split q again in every tile)
+#pragma unroll
+    for (int i = 0; i < QP; ++i)
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk) asm volatile("" : "+v"(qop[i][kk]));
+  }
+
+  // Piece c of the thread: K pieces first, then V, in steps of GT / SL keys; its slot is the
+  // same in all.  The row offset of the tile after is looked up one load earlier (a
+  // block-table entry arrives meanwhile).
+  constexpr int NK = PC / GT;  // K pieces of a thread
+  const int psl = tid % SL, pkey0 = tid / SL;
+  auto piece_is_v = [&](int c) { return c >= NK; };
+  auto piece_key = [&](int c) { return pkey0 + c % NK * (GT / SL); };
+  // (scales as whole words, whose byte is taken at the store: a byte load is extended at once,
+  // which waits for it)
+  uint32_t code[NP], scale[NP];
+  auto scale_byte = [&](int c) { return (scale[c] >> (8 * ((piece_key(c) * GR + psl / 4) & 3))) & 0xFFu; };
+  TileWalk walk(p.kv, b, g, lane);
+  auto tile_off = [&](int t) { return walk(min(t, ntiles - 1)); };
+  const uint32_t code_at = static_cast<uint32_t>(pkey0 * (D / 2) + 4 * psl);
+  const uint32_t scale_at = static_cast<uint32_t>((pkey0 * GR + psl / 4) & ~3);
+  auto load_tile = [&](int64_t off) {
+    // (descriptors of the tile: the address arithmetic is scalar)
+    auto tile = [&](const uint8_t* base, int64_t at, int bytes) {
+      return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(base + at), 0, bytes, kRawBufferFlags);
+    };
+    const uint64_t uoff = static_cast<uint64_t>(off);
+    const auto kc = tile(p.kc, uoff >> 1, kStep * D / 2), ks = tile(p.ks, uoff >> 5, kStep * GR);
+    const auto vc = tile(p.vc, uoff >> 1, kStep * D / 2), vs = tile(p.vs, uoff >> 5, kStep * GR);
+#pragma unroll
+    for (int c = 0; c < NP; ++c) {
+      const uint32_t keys = c % NK * (GT / SL);
+      code[c] = __builtin_amdgcn_raw_buffer_load_b32(piece_is_v(c) ? vc : kc, code_at + keys * (D / 2), 0, 0);
+      scale[c] = __builtin_amdgcn_raw_buffer_load_b32(piece_is_v(c) ? vs : ks, scale_at + keys * GR, 0, 0);
+    }
+  };
+  // every key group goes through as many tiles as the first (those past the last key's hold
+  // no live key), so that all threads meet at the same barriers
+  const int nu = (ntiles + KS - 1) / KS;
+  int64_t next_off = 0;
+  if (nu > 0) {
+    load_tile(tile_off(kg));
+    next_off = tile_off(kg + KS);
+  }
+
+  // the block's scales of V: the largest and the first NaN of each group
+  if (threadIdx.x < GR) {
+    s_top[threadIdx.x] = 0;
+    s_nan[threadIdx.x] = 0x7FFFFFFF;
+  }
+  __syncthreads();
+  {
+    constexpr int PS = 2 * GR;          // 16-byte pieces of a step's scales
+    constexpr int KW = 4 / GR;          // keys of a word
+    auto scan = [&](auto&& each) {      // each(word, its first key)
+      for (int i = threadIdx.x; i < ntiles * PS; i += NT) {
+        const int step = i / PS, part = i % PS;
+        const uint4 v = *reinterpret_cast<const uint4*>(p.vs + p.kv.Row(b, g, static_cast<int64_t>(kStep) * step) / 32 + 16 * part);
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int key = kStep * step + (4 * part + e) * KW;
+          each(w[e] & (key >= kend ? 0u : (KW == 2 && key + 1 >= kend) ? 0xFFFFu : ~0u), key);
+        }
+      }
+    };
+    uint32_t even = 0, odd = 0;  // two bytes of each word as 16-bit values
+    scan([&](uint32_t w, int) {
+      even = max_u16x2(even, w & 0x00FF00FFu);
+      odd = max_u16x2(odd, (w >> 8) & 0x00FF00FFu);
+    });
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+      even = max_u16x2(even, static_cast<uint32_t>(__shfl_xor(static_cast<int>(even), o)));
+      odd = max_u16x2(odd, static_cast<uint32_t>(__shfl_xor(static_cast<int>(odd), o)));
+    }
+    if (lane == 0) {
+      const uint32_t m[4] = {even & 0xFFFFu, odd & 0xFFFFu, even >> 16, odd >> 16};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) atomicMax(&s_top[e % GR], m[e]);
+    }
+    __syncthreads();
+    uint32_t any = 0;
+#pragma unroll
+    for (int e = 0; e < GR; ++e) any = max(any, s_top[e]);
+    if (any >= kScaleNan) {  // again, byte by byte (block-uniform)
+      __syncthreads();
+      if (threadIdx.x < GR) s_top[threadIdx.x] = 0;
+      __syncthreads();
+      scan([&](uint32_t w, int key) {
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t x = (w >> (8 * e)) & 0xFFu;
+          if (x >= kScaleNan) atomicMin(&s_nan[e % GR], key + e / GR);
+          else atomicMax(&s_top[e % GR], x);
+        }
+      });
+      __syncthreads();
+    }
+  }
+
+  // (buffer of the group's u-th tile)
+  auto tile_k = [&](int u) { return smem_w + (kg * NB + (u & (NB - 1))) * 2 * kTileBytes; };
+  auto tile_v = [&](int u) { return tile_k(u) + kTileBytes; };
+  const int v_add = kVTop - static_cast<int>(s_top[psl / 4]);  // to a V piece's scale byte
+  auto store_tile = [&](int u) {
+    const int t = u * KS + kg;
+#pragma unroll
+    for (int c = 0; c < NP; ++c) {
+      const int key = piece_key(c);
+      const uint32_t sb = scale_byte(c);
+      uint32_t w[4];
+      if (!piece_is_v(c)) {
+        fp4_to_bf16(code[c], e8m0_scale_or_nan(sb), w);
+        *reinterpret_cast<uint4*>(tile_k(u) + key * (2 * D) + 16 * k_slot<SL>(key, psl)) = make_uint4(w[0], w[1], w[2], w[3]);
+      } else {
+        const bool dead = (sb >= kScaleNan) | (kStep * t + key >= kend);
+        if constexpr (F32) {
+          fp4_to_bf16(code[c], e8m0_scale(dead ? 0u : sb), w);
+        } else {
+          const float s = e8m0_scale(static_cast<uint32_t>(max(static_cast<int>(dead ? 0u : sb) + (dead ? 0 : v_add), 0)));
+          w[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(code[c], s, 0));
+          w[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(code[c], s, 1));
+          w[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(code[c], s, 2));
+          w[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(code[c], s, 3));
+        }
+        *reinterpret_cast<uint4*>(tile_v(u) + key * (2 * D) + 16 * v_slot<SL>(key, psl)) = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+    }
+  };
+
+  float m_run = -INFINITY, l_run = 0.0f;
+  f32x16_t o[DT];  // O^T[32 dt + 8 (r >> 2) + 4 h + (r & 3)][column j]
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) o[dt][r] = 0.0f;
+
+  f32x16_t acc;                                  // scores
+  uint32_t pw[F32 ? 3 : 1][2][4];                // P operand: parts, chunks of 16 keys
+  auto softmax = [&](int u) {
+    const int t = u * KS + kg;
+    if (kStep * t + kStep > least) {  // some column of the wave ends in or before this tile
+      asm volatile("");               // (a branch: not selects in every tile)
+      const int32_t base = kStep * t + 4 * h;
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        if (base + 8 * (r >> 2) + (r & 3) >= limit) acc[r] = -INFINITY;
+    }
+    float bm = acc[0];
+#pragma unroll
+    for (int r = 1; r < 16; ++r) bm = fmaxf(bm, acc[r]);
+    const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(bm), __float_as_uint(bm), false, false);
+    bm = fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1]));
+    const float mn = fmaxf(m_run, bm * p.scale);
+    if (__builtin_amdgcn_ballot_w64(mn > m_run) != 0) {
+      const float cf = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m_run - mn);
+      l_run *= cf;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[dt][r] *= cf;
+      m_run = mn;
+    }
+    const float sub = (F32 ? 0.0f : kPBias) - (m_run == -INFINITY ? 0.0f : m_run);
+#pragma unroll
+    for (int r = 0; r < 16; r += 2) {
+      float v0 = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[r], p.scale, sub));
+      float v1 = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[r + 1], p.scale, sub));
+      if constexpr (F32) {
+        l_run += v0;
+        l_run += v1;
+#pragma unroll
+        for (int i = 0; i < 3; ++i) {
+          const uint32_t w = __builtin_bit_cast(uint32_t, bf16x2_t{static_cast<__bf16>(v0), static_cast<__bf16>(v1)});
+          pw[i][r / 8][(r % 8) / 2] = w;
+          v0 -= __uint_as_float(w << 16);
+          v1 -= __uint_as_float(w & 0xFFFF0000u);
+        }
+      } else {
+        const f16x2_t v = {static_cast<_Float16>(v0), static_cast<_Float16>(v1)};
+        l_run = __builtin_amdgcn_fdot2(v, f16x2_t{static_cast<_Float16>(1.0f), static_cast<_Float16>(1.0f)}, l_run, false);
+        pw[0][r / 8][(r % 8) / 2] = __builtin_bit_cast(uint32_t, v);
+      }
+    }
+  };
+  // A operand of V^T: lane (row, h) of output tile dt and k slots of chunk c: keys 16 c + 8 q +
+  // 4 h .. +4, which the 16 lanes of a transposed read bring as 4 keys x 16 dimensions
+  const int tkey = 4 * h + ((lane & 15) >> 2), tdim = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+  auto read_v = [&](int u, int c, s16x4_t (&part)[DT][2]) {
+    const uint8_t* vt = tile_v(u);
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        const int key = 16 * c + 8 * q + tkey, slot = (32 * dt + tdim) >> 3;
+        const uint8_t* at = vt + key * (2 * D) + 16 * v_slot<SL>(key, slot) + 2 * (tdim & 7);
+        part[dt][q] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4_t*)(at));
+      }
+  };
+  auto products = [&](int c, const s16x4_t (&part)[DT][2]) {
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) {
+      const auto a = __builtin_shufflevector(part[dt][0], part[dt][1], 0, 1, 2, 3, 4, 5, 6, 7);
+      if constexpr (F32) {
+#pragma unroll
+        for (int i = 2; i >= 0; --i)
+          o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+              __builtin_bit_cast(bf16x8_t, a),
+              __builtin_bit_cast(bf16x8_t, make_uint4(pw[i][c][0], pw[i][c][1], pw[i][c][2], pw[i][c][3])), o[dt], 0, 0, 0);
+      } else {
+        o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
+            __builtin_bit_cast(f16x8_t, a),
+            __builtin_bit_cast(f16x8_t, make_uint4(pw[0][c][0], pw[0][c][1], pw[0][c][2], pw[0][c][3])), o[dt], 0, 0, 0);
+      }
+    }
+  };
+  auto read_k = [&](int u, int kk) {
+    return *reinterpret_cast<const bf16x8_t*>(tile_k(u) + j * (2 * D) + 16 * k_slot<SL>(j, 2 * kk + h));
+  };
+  auto score = [&](int kk, bf16x8_t k) {
+#pragma unroll
+    for (int i = QP - 1; i >= 0; --i) acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k, qop[i][kk], acc, 0, 0, 0);
+  };
+  // M of tile u: P V of tile u - 1 and K Q^T of tile u.  Its operands are read ahead, so that
+  // the products do not wait for LDS (fp32 q leaves no registers for that: read_m does nothing).
+  s16x4_t vop[F32 ? 1 : 2][DT][2];
+  bf16x8_t kop[F32 ? 1 : D / 16];
+  auto read_m = [&](int u, bool pv, bool qk) {
+    if constexpr (!F32) {
+      if (pv) {
+        read_v(u - 1, 0, vop[0]);
+        read_v(u - 1, 1, vop[1]);
+      }
+      if (qk) {
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) kop[kk] = read_k(u, kk);
+      }
+    }
+  };
+  auto multiply = [&](int u, bool pv, bool qk) {
+    if (pv) {
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        if constexpr (F32) read_v(u - 1, c, vop[0]);
+        products(c, vop[F32 ? 0 : c]);
+      }
+    }
+    if (qk) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[r] = 0.0f;
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk) {
+        if constexpr (F32) score(kk, read_k(u, kk));
+        else score(kk, kop[kk]);
+      }
+    }
+  };
+
+  // A wave alternates between vector work (V: the softmax of its group's tile u, and its share
+  // of the staging) and products (M: P V of tile u, K Q^T of tile u + 1).  Between two barriers
+  // the first group does V then M, and the second, which shares every SIMD with it, M (of the
+  // tile before) then V: while one wave of a SIMD multiplies the other exponentiates.  In phase
+  // (every wave V then M, a barrier a tile) 2048 rows at 6144 keys took 329 us, so 294.
+  // Interval u stores tile u + 2.  K of tile x is read in interval x - 1 (ahead of x in the
+  // second group), its V in x or x + 1: four buffers.
+  // (kg as a lane value: as a scalar one the loops' registers spill)
+  const bool second = threadIdx.x >= GT;
+  auto interval_end = [&]() {  // (nothing moves over it: the scheduler would mix the intervals' arithmetic)
+    __builtin_amdgcn_sched_barrier(0);
+    lds_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  if (nu > 0) {
+    auto load_next = [&](int u) {
+      if (u < nu) {
+        load_tile(next_off);
+        next_off = tile_off((u + 1) * KS + kg);
+      }
+    };
+    auto vector_work = [&](int u) {
+      softmax(u);
+      if (u + 2 < nu) store_tile(u + 2);
+      load_next(u + 3);
+    };
+    store_tile(0);
+    load_next(1);
+    if (nu > 1) store_tile(1);
+    load_next(2);
+    interval_end();
+    read_m(0, false, true);
+    multiply(0, false, true);
+    if (second) {
+      vector_work(0);
+      read_m(1, true, nu > 1);
+      interval_end();
+      for (int u = 1; u < nu; ++u) {
+        multiply(u, true, true);
+        __builtin_amdgcn_sched_barrier(0);
+        vector_work(u);
+        read_m(u + 1, true, true);  // (the last K is not used: a tile's buffer all the same)
+        interval_end();
+      }
+    } else {
+      for (int u = 0; u + 1 < nu; ++u) {
+        read_m(u + 1, true, true);
+        __builtin_amdgcn_sched_barrier(0);
+        vector_work(u);
+        __builtin_amdgcn_sched_barrier(0);
+        multiply(u + 1, true, true);
+        interval_end();
+      }
+      read_m(nu, true, false);
+      vector_work(nu - 1);
+      interval_end();
+    }
+    multiply(nu, true, false);
+  }
+
+  // column j's sum over its two lanes, and the key groups' states
+  l_run += xor_lane<32>(l_run, lane);
+  {
+    lds_barrier();  // both groups are done with their tiles
+    float* rec = reinterpret_cast<float*>(smem_w) + wave * OW * 64 + lane;
+    if (kg > 0) {
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) rec[(dt * 16 + r) * 64] = o[dt][r];
+      rec[DT * 16 * 64] = m_run;
+      rec[(DT * 16 + 1) * 64] = l_run;
+    }
+    __syncthreads();
+    if (kg > 0) return;
+    const float m2 = rec[DT * 16 * 64], l2 = rec[(DT * 16 + 1) * 64];
+    const float mn = fmaxf(m_run, m2), top = mn == -INFINITY ? 0.0f : mn;
+    const float f1 = __builtin_amdgcn_exp2f(m_run - top), f2 = __builtin_amdgcn_exp2f(m2 - top);
+    l_run = l_run * f1 + l2 * f2;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) {
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[dt][r] = o[dt][r] * f1 + rec[(dt * 16 + r) * 64] * f2;
+    }
+  }
+  if (!mine) return;
+  const float inv = l_run == 0.0f ? 0.0f : 1.0f / l_run;
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt) {
+    const bool bad = s_nan[dt] < limit;
+    const int back = static_cast<int>(s_top[dt]) - kVTop;
+#pragma unroll
+    for (int r4 = 0; r4 < 4; ++r4) {
+      f32x4_t v;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        v[e] = o[dt][4 * r4 + e] * inv;
+        if constexpr (!F32) v[e] = __builtin_ldexpf(v[e], back);
+        if (bad) v[e] = __builtin_nanf("");
+      }
+      const int64_t to = qrow + 32 * dt + 8 * r4 + 4 * h;
+      if constexpr (F32) {
+        *reinterpret_cast<f32x4_t*>(static_cast<float*>(p.out) + to) = v;
+      } else {
+        const uint32_t w0 = f32_to_bf16_bits(v[0]) | (static_cast<uint32_t>(f32_to_bf16_bits(v[1])) << 16);
+        const uint32_t w1 = f32_to_bf16_bits(v[2]) | (static_cast<uint32_t>(f32_to_bf16_bits(v[3])) << 16);
+        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + to) = make_uint2(w0, w1);
+      }
+    }
+  }
+}
+
 constexpr int kWaves = 8;
 constexpr int64_t kMaxRows = 65535;  // query rows of a call
 
@@ -569,7 +1087,31 @@ int64_t WorkspaceBytes(int64_t units, int64_t qt, int64_t G, int64_t hkv, int64_
 }
 
 template <int D, bool F32>
+void LaunchWide(Attn4Args p, hipStream_t s) {
+  p.qt = 32 / p.G;
+  p.tiles = static_cast<int32_t>(CeilDiv(p.seq, kWideWaves * p.qt));
+  p.units = p.batch * p.tiles;
+  p.tiles_inv = static_cast<uint32_t>(CeilDiv(int64_t{1} << 32, p.tiles));
+  const dim3 grid(static_cast<unsigned>(p.hkv), static_cast<unsigned>(p.units));
+  RecordLaunch(static_cast<int64_t>(grid.x) * grid.y, 512, 0, "kv4_attention_wide<%s,d=%d>", F32 ? "f32" : "bf16", D);
+  hipLaunchKernelGGL((kv4_attention_wide_kernel<D, F32>), grid, dim3(512), 0, s, p);
+}
+
+// The kernel for many rows where its blocks occupy enough of the CUs (one each) and a sequence
+// fills at least one: its blocks walk their keys whole, while the other kernel's pieces fill
+// the CUs at any shape.  32 q / 8 kv heads, d = 128 (us, this kernel / the other): 128 blocks (512
+// rows) 18.5 / 19.2, 80 blocks (300 rows) 15 / 12.8, 256 blocks (1000 rows) 29 / 41; 16 sequences of
+// one row at 4200-8320 keys (128 blocks of one live column group in eight) 273 / 31; fp32 q does
+// three products for one here: 128 blocks (512 rows at 2048 keys) 94 / 85.
+template <bool F32>
+bool ManyRows(const Attn4Args& p) {
+  const int64_t rows = kWideWaves * (32 / p.G), blocks = p.batch * CeilDiv(p.seq, rows) * p.hkv, cus = DeviceCUs();
+  return p.seq >= rows && (F32 ? 4 : 2) * blocks >= (F32 ? 3 : 1) * cus;
+}
+
+template <int D, bool F32>
 void Launch(const Attn4Args& p, hipStream_t s) {
+  if (ManyRows<F32>(p)) return LaunchWide<D, F32>(p, s);
   // kv head fastest: with 8 kv heads every block of a head runs on one XCD
   const dim3 grid(static_cast<unsigned>(p.hkv), static_cast<unsigned>(p.slots > 0 ? p.slots : p.units));
   constexpr int NW = kWaves;

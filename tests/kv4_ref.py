@@ -97,8 +97,11 @@ def attention(q, k, v, start, lens, scale):
 def attention_bound(out, mag, top, keys, d, dtype):
     """What |kernel - out| may be: the rounding of out, and relative errors of the probabilities: fp32
     sums of d products in the scores (each off by at most (d + 4) 2^-24 sum|qk|, in the exponent, in numerator and
-    denominator), exp2 (2 ulp), their parts (bf16 hi + lo: 2^-16; three parts: 2^-24) and fp32 sums over the keys."""
-    parts = 2.0**-16 if dtype == "bf16" else 2.0**-23
+    denominator), exp2 (2 ulp), their parts and fp32 sums over the keys.  Parts: bf16 hi + lo 2^-16, three parts 2^-23;
+    the kernel for many rows takes bf16 calls' probabilities in f16, off by at most half a step, 2^-11, each, in the
+    numerator and in the row sum, which adds the same rounded values."""
+    wide = N.last_launch().kernel.startswith(b"kv4_attention_wide")
+    parts = (2 * 2.0**-11 if wide else 2.0**-16) if dtype == "bf16" else 2.0**-23
     rel = 2 * (d + 4) * 2.0**-24 * top + 4 * 2.0**-23 + parts + 2 * (keys + 64) * 2.0**-24
     return HALF[dtype] * out.abs() * 1.001 + rel * mag + 1e-30
 

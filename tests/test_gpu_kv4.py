@@ -486,6 +486,70 @@ def test_attention_shared_prefix_stride_zero():
         assert ((out[i].double() - want.flatten()).abs() <= bound).all() and ((one[0].double() - want.flatten()).abs() <= bound).all()
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("hq,hkv,d,b,n,start,lens,block", [
+    (64, 16, 128, 2, 200, [0, 70], None, 0),
+    (64, 16, 64, 2, 200, [0, 70], [200, 77], 32),
+    (32, 32, 128, 1, 800, [5], None, 64),               # heads of their own
+    (48, 16, 128, 1, 490, [33], None, 0),               # three heads a group: columns to spare
+    (80, 16, 64, 1, 300, [0], None, 0),                 # five
+    (14, 2, 64, 9, 180, [0, 3, 90, 0, 50, 7, 8, 9, -40], [180, 1, 180, 0, 44, 180, 2, 33, 90], 32),
+    (64, 64, 128, 1, 300, [-30], None, 0),              # rows before position 0
+    (64, 64, 64, 1, 300, [20], None, 0),                # past the cache
+    (256, 16, 64, 1, 100, [0], None, 0),                # sixteen heads a group
+    (32, 8, 128, 16, 33, [31 * i for i in range(16)], [33 - 2 * i for i in range(16)], 32),  # a second block of one row
+])
+def test_attention_many_rows(dtype, hq, hkv, d, b, n, start, lens, block):
+    cap = 160 if start == [20] else max(max(s + n for s in start), 32) + 31
+    attention_case(n, b, n, hq, hkv, d, cap - cap % 32, start, lens=lens, block=block, dtype=dtype)
+    assert N.last_launch().kernel.startswith(b"kv4_attention_wide")
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_attention_many_rows_spread_values(dtype):
+    """values whose scales differ widely between keys and between groups, rows that meet only the small ones"""
+    g, n, hq, hkv, d, cap = gen_of(3), 400, 64, 16, 128, 416
+    c = Cache(1, hkv, cap, d)
+    k, v = randn(g, 1, hkv, cap, d), randn(g, 1, hkv, cap, d)
+    v *= torch.exp2(torch.randint(-12, 13, (1, hkv, cap, 4), generator=g, device="cuda").double()).float().repeat_interleave(32, -1)
+    v[..., :32] *= 2.0**60
+    v[..., 32:64] *= 2.0**-60
+    v[:, :, :50, 64:96] = 0  # a group of zeros first
+    c.put_values("k", k)
+    c.put_values("v", v)
+    q = randn(g, n, hq * d).to(DTYPES[dtype][0])
+    out, ws = torch.empty_like(q), R.workspace(1, n, hq, hkv, d, cap)
+    R.attend(c, q, out, 1, n, hq, i64(0), ws, dtype=dtype)
+    assert N.last_launch().kernel.startswith(b"kv4_attention_wide")
+    want, mag, top = R.attention(q.double().view(1, n, hq, d), c.values("k"), c.values("v"), [0], [n], R.softmax_scale(d))
+    assert ((out.double().view_as(want) - want).abs() <= R.attention_bound(want, mag, top, cap, d, dtype)).all()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("d", [64, 128])
+def test_attention_many_rows_nan(dtype, d):
+    """as test_attention_nan_keys_and_values, for the kernel of many rows"""
+    g, hq, hkv, n, start, cap = gen_of(7), 64, 16, 400, 40, 480
+    for which in ("k", "v"):
+        c = Cache(1, hkv, cap, d, 32)
+        for m in ("k", "v"):
+            c.put_values(m, randn(g, 1, hkv, cap, d))
+        clean = {m: c.values(m) for m in ("k", "v")}
+        marks = {m: c.whole(m + "s") for m in ("k", "v")}
+        marks[which][0, 3, 100, 1] = 253  # seen by rows 60 and later of kv head 3
+        marks[which][0, 5, start + n :] = 255  # behind every row
+        c.put(which + "s", marks[which])
+        q = randn(g, n, hq * d).to(DTYPES[dtype][0])
+        out = torch.empty_like(q)
+        R.attend(c, q, out, 1, n, hq, i64(start), R.workspace(1, n, hq, hkv, d, cap), dtype=dtype)
+        want, mag, top = R.attention(q.double().view(1, n, hq, d), clean["k"], clean["v"], [start], [n], R.softmax_scale(d))
+        bad = torch.zeros(n, hq, d, dtype=torch.bool, device="cuda")
+        bad[60:, 12:16, slice(32, 64) if which == "v" else slice(None)] = True
+        got = out.view(n, hq, d)
+        assert torch.equal(torch.isnan(got), bad)
+        assert (((got.double() - want[0]).abs() <= R.attention_bound(want, mag, top, cap, d, dtype)[0]) | bad).all()
+
+
 # ------------------------------------------------------------------ together
 class Model:
     """One attention layer of a decode: append of a token of each sequence, then attention over the cache."""
