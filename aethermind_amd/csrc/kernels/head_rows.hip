@@ -49,7 +49,7 @@ struct HeadRowArgs {
   uint8_t *ksc, *vsc;
   int32_t* err;
   KvRows kv;
-  uint32_t rows, seq, hq, hk, hv, chunks;  // hv: 0 for norm_rope
+  uint32_t rows, seq, hq, hk, hv;  // hv: 0 for norm_rope
   int32_t d;
   float eps;
 };
@@ -103,20 +103,30 @@ __device__ __forceinline__ void unpack8(const Raw8<A>& r, float (&v)[8]) {
     }
   }
 }
+// One rounding to the type.  bf16: the conversion of two values at once, which is
+// f32_to_bf16_bits but for the pattern of a NaN; those take the branch.
 template <class A>
 __device__ __forceinline__ Raw8<A> pack8(const float (&v)[8]) {
   Raw8<A> r;
+  if constexpr (A::kDtype == AM_DT_BF16) {
+    float t = 0.0f;  // NaN where a value is NaN or infinite
 #pragma unroll
-  for (size_t i = 0; i < sizeof(r) / 16; ++i) {
+    for (int e = 0; e < 8; ++e) t = __builtin_fmaf(v[e], 0.0f, t);
     uint32_t w[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      if constexpr (A::kDtype == AM_DT_BF16)
+    for (int e = 0; e < 4; ++e)
+      w[e] = __builtin_bit_cast(uint32_t, bf16x2_t{static_cast<__bf16>(v[2 * e]), static_cast<__bf16>(v[2 * e + 1])});
+    if (__builtin_expect(t != t, 0)) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
         w[e] = f32_to_bf16_bits(v[2 * e]) | (static_cast<uint32_t>(f32_to_bf16_bits(v[2 * e + 1])) << 16);
-      else
-        w[e] = __float_as_uint(v[4 * i + e]);
     }
-    r.w[i] = make_uint4(w[0], w[1], w[2], w[3]);
+    r.w[0] = make_uint4(w[0], w[1], w[2], w[3]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      r.w[i] = make_uint4(__float_as_uint(v[4 * i]), __float_as_uint(v[4 * i + 1]), __float_as_uint(v[4 * i + 2]),
+                          __float_as_uint(v[4 * i + 3]));
   }
   return r;
 }
@@ -153,23 +163,22 @@ __device__ __forceinline__ double lanes_sum(double v) {
 
 // Norm (gain w, or none) and rotation of one head's row: lane `sub` of LP holds values
 // 8 sub .. +8 of each half, so a pair's two values are in one lane.
-template <class F, int D, class A, bool VEC>
-__device__ __forceinline__ void norm_rotate(float (&lo)[8], float (&hi)[8], const void* gain, float eps, int sub,
+template <class F, int D, class A>
+__device__ __forceinline__ void norm_rotate(float (&lo)[8], float (&hi)[8], bool norm, const Raw8<A> (&gain)[2], float eps,
                                             const float (&c)[8], const float (&s)[8], bool turn) {
   constexpr int LP = D / 16;
   F x1[8], x2[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) x1[i] = lo[i], x2[i] = hi[i];
-  if (gain != nullptr) {
+  if (norm) {
     F ss = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) ss = fma(x1[i], x1[i], fma(x2[i], x2[i], ss));
     ss = lanes_sum<LP>(ss);
     const F inv = F(1) / sqrt(ss / F(D) + F(eps));
-    const auto* w = static_cast<const typename A::T*>(gain) + 8 * sub;
     float w1[8], w2[8];
-    unpack8<A>(load_raw8<A, VEC>(w), w1);
-    unpack8<A>(load_raw8<A, VEC>(w + D / 2), w2);
+    unpack8<A>(gain[0], w1);
+    unpack8<A>(gain[1], w2);
 #pragma unroll
     for (int i = 0; i < 8; ++i) x1[i] = x1[i] * inv * F(w1[i]), x2[i] = x2[i] * inv * F(w2[i]);
   }
@@ -226,86 +235,67 @@ __device__ __forceinline__ bool row_position(const HeadRowArgs& p, uint32_t row,
 }
 
 // D in {64, 128, 256}: LP = D / 16 lanes own a row of a head, 8 values of each half per
-// lane (two 16-byte loads of bf16).  A lane group takes HB heads of one token row, with the
-// table row read once and all heads' loads in flight.
-template <class A, int D, int MODE, bool VEC, int HB>
+// lane (two 16-byte loads of bf16), and every row of a head its own lanes: 2048 rows of 32 + 8
+// heads of 128 (43 MB) take 8.9 us, 4.8 TB/s, a copy's rate; two heads per lane group, the
+// table row read once, 9.9, four 11.0; one row 2.3, 2.9 and 3.8.
+template <class A, int D, int MODE, bool VEC>
 __global__ __launch_bounds__(256) void head_rows_kernel(HeadRowArgs p) {
   constexpr int LP = D / 16;
   using T = typename A::T;
-  const uint32_t group = blockIdx.x * (256 / LP) + threadIdx.x / LP;
+  const uint32_t item = blockIdx.x * (256 / LP) + threadIdx.x / LP;
   const int sub = threadIdx.x % LP;
-  const uint32_t row = group / p.chunks, first = (group - row * p.chunks) * HB;
+  const uint32_t heads = p.hq + p.hk + p.hv;
+  const uint32_t row = item / heads, h = item - row * heads;
   if (row >= p.rows) return;
   uint32_t b;
   int64_t at;
   bool ok;
   if (!row_position<MODE>(p, row, b, at, ok)) return;
-  const uint32_t heads = p.hq + p.hk + p.hv;
-  Raw8<A> lo[HB], hi[HB];
-#pragma unroll
-  for (int u = 0; u < HB; ++u) {
-    const uint32_t h = min(first + u, heads - 1);
-    const T* x = h < p.hq          ? static_cast<const T*>(p.q) + row * p.qs + h * D
-                 : h < p.hq + p.hk ? static_cast<const T*>(p.k) + row * p.ks + (h - p.hq) * D
-                                   : static_cast<const T*>(p.v) + row * p.vs + (h - p.hq - p.hk) * D;
-    lo[u] = load_raw8<A, VEC>(x + 8 * sub);
-    hi[u] = load_raw8<A, VEC>(x + D / 2 + 8 * sub);
+  const bool is_q = h < p.hq, is_k = !is_q && h < p.hq + p.hk;
+  const uint32_t g = is_q ? h : is_k ? h - p.hq : h - p.hq - p.hk;
+  const T* x = static_cast<const T*>(is_q ? p.q : is_k ? p.k : p.v) + row * (is_q ? p.qs : is_k ? p.ks : p.vs) + g * D + 8 * sub;
+  Raw8<A> lo = load_raw8<A, VEC>(x), hi = load_raw8<A, VEC>(x + D / 2);
+  const T* w = static_cast<const T*>(is_q ? p.q_w : is_k ? p.k_w : nullptr);
+  Raw8<A> gain[2];
+  if (w != nullptr) {
+    gain[0] = load_raw8<A, VEC>(w + 8 * sub);
+    gain[1] = load_raw8<A, VEC>(w + D / 2 + 8 * sub);
   }
   float c[8], s[8];
-  {
+  if (MODE == kNormRope || is_q || is_k) {
     const int64_t t = (ok ? at : 0) * (D / 2) + 8 * sub;
     unpack8<ActF32>(load_raw8<ActF32, VEC>(p.cos_tab + t), c);
     unpack8<ActF32>(load_raw8<ActF32, VEC>(p.sin_tab + t), s);
   }
-  // the cache row of head 0 (-1: none to write); the other heads' rows follow at one distance
-  int64_t dst0 = -1, head_step = 0;
-  if constexpr (MODE != kNormRope) {
+  float x1[8], x2[8];
+  unpack8<A>(lo, x1);
+  unpack8<A>(hi, x2);
+  if (MODE == kNormRope || is_q) {
+    norm_rotate<float, D, A>(x1, x2, w != nullptr, gain, p.eps, c, s, ok);
+    T* out = (is_q ? static_cast<T*>(p.q_out) + row * p.qos : static_cast<T*>(p.k_out) + row * p.kos) + g * D + 8 * sub;
+    store_raw8<A, VEC>(out, pack8<A>(x1));
+    store_raw8<A, VEC>(out + D / 2, pack8<A>(x2));
+  } else if constexpr (MODE != kNormRope) {
     if (!ok && p.err != nullptr) *p.err = 1;
-    if (ok) dst0 = p.kv.WriteRow(b, 0, at);
-    head_step = (p.kv.table == nullptr ? p.kv.cap : int64_t{1} << p.kv.shift) * D;
-  }
-#pragma unroll
-  for (int u = 0; u < HB; ++u) {
-    const uint32_t h = first + u;
-    if (h >= heads) return;
-    if (h < p.hq || (MODE == kNormRope && h < p.hq + p.hk)) {
-      const bool is_q = h < p.hq;
-      float x1[8], x2[8];
-      unpack8<A>(lo[u], x1);
-      unpack8<A>(hi[u], x2);
-      norm_rotate<float, D, A, VEC>(x1, x2, is_q ? p.q_w : p.k_w, p.eps, sub, c, s, ok);
-      T* out = (is_q ? static_cast<T*>(p.q_out) + row * p.qos + h * D : static_cast<T*>(p.k_out) + row * p.kos + (h - p.hq) * D) + 8 * sub;
-      store_raw8<A, VEC>(out, pack8<A>(x1));
-      store_raw8<A, VEC>(out + D / 2, pack8<A>(x2));
-    } else if constexpr (MODE != kNormRope) {
-      const bool is_k = h < p.hq + p.hk;
-      const uint32_t g = h - p.hq - (is_k ? 0 : p.hk);
-      if (dst0 < 0) continue;
-      const int64_t dst = dst0 + g * head_step;
-      if constexpr (MODE == kAppendPlain) {
-        T* out = static_cast<T*>(is_k ? p.kc : p.vc) + dst + 8 * sub;
-        if (is_k) {
-          float x1[8], x2[8];
-          unpack8<A>(lo[u], x1);
-          unpack8<A>(hi[u], x2);
-          norm_rotate<float, D, A, VEC>(x1, x2, p.k_w, p.eps, sub, c, s, true);
-          lo[u] = pack8<A>(x1);
-          hi[u] = pack8<A>(x2);
-        }
-        store_raw8<A, VEC>(out, lo[u]);
-        store_raw8<A, VEC>(out + D / 2, hi[u]);
-      } else {
-        float x1[8], x2[8];
-        unpack8<A>(lo[u], x1);
-        unpack8<A>(hi[u], x2);
-        // 64 bits: a key next to a code's border takes the same code whatever the order of
-        // the sums (fp32 errors of 2^-24 move about one code in 10^6)
-        if (is_k) norm_rotate<double, D, A, VEC>(x1, x2, p.k_w, p.eps, sub, c, s, true);
-        uint8_t* codes = static_cast<uint8_t*>(is_k ? p.kc : p.vc) + dst / 2 + 4 * sub;
-        uint8_t* scales = (is_k ? p.ksc : p.vsc) + dst / 32 + sub / 4;
-        kv4_store8(x1, sub, codes, scales);
-        kv4_store8(x2, sub, codes + D / 4, scales + D / 64);
+    const int64_t dst = ok ? p.kv.WriteRow(b, g, at) : -1;
+    if (dst < 0) return;
+    if constexpr (MODE == kAppendPlain) {
+      if (is_k) {
+        norm_rotate<float, D, A>(x1, x2, w != nullptr, gain, p.eps, c, s, true);
+        lo = pack8<A>(x1);
+        hi = pack8<A>(x2);
       }
+      T* out = static_cast<T*>(is_k ? p.kc : p.vc) + dst + 8 * sub;
+      store_raw8<A, VEC>(out, lo);
+      store_raw8<A, VEC>(out + D / 2, hi);
+    } else {
+      // 64 bits: a key next to a code's border takes the same code whatever the order of the
+      // sums (fp32 errors of 2^-24 move about one code in 10^6)
+      if (is_k) norm_rotate<double, D, A>(x1, x2, w != nullptr, gain, p.eps, c, s, true);
+      uint8_t* codes = static_cast<uint8_t*>(is_k ? p.kc : p.vc) + dst / 2 + 4 * sub;
+      uint8_t* scales = (is_k ? p.ksc : p.vsc) + dst / 32 + sub / 4;
+      kv4_store8(x1, sub, codes, scales);
+      kv4_store8(x2, sub, codes + D / 4, scales + D / 64);
     }
   }
 }
@@ -372,19 +362,13 @@ constexpr int64_t kMaxItems = int64_t{1} << 26;  // head rows of a call (a grid 
 
 const char* const kModeName[] = {"qk_norm_rope", "kv_append", "kv_append_kv4"};
 
-template <class A, int D, int MODE, bool VEC, int HB>
-void LaunchHeadRows(HeadRowArgs p, hipStream_t s) {
-  p.chunks = static_cast<uint32_t>(CeilDiv(p.hq + p.hk + p.hv, HB));
-  const int64_t grid = CeilDiv(static_cast<int64_t>(p.rows) * p.chunks, 256 / (D / 16));
-  RecordLaunch(grid, 256, 0, "%s<%s,d=%d,vec=%d,hb=%d>", kModeName[MODE], A::kDtype == AM_DT_BF16 ? "bf16" : "f32", D,
-               VEC ? 1 : 0, HB);
-  hipLaunchKernelGGL((head_rows_kernel<A, D, MODE, VEC, HB>), dim3(static_cast<unsigned>(grid)), dim3(256), 0, s, p);
-}
-
 template <class A, int MODE, int D>
-void LaunchHeadRowsD(const HeadRowArgs& p, bool vec, hipStream_t s) {
-  if (!vec) return LaunchHeadRows<A, D, MODE, false, 1>(p, s);
-  LaunchHeadRows<A, D, MODE, true, 1>(p, s);
+void LaunchHeadRows(const HeadRowArgs& p, bool vec, hipStream_t s) {
+  const int64_t grid = CeilDiv(static_cast<int64_t>(p.rows) * (p.hq + p.hk + p.hv), 256 / (D / 16));
+  RecordLaunch(grid, 256, 0, "%s<%s,d=%d,vec=%d>", kModeName[MODE], A::kDtype == AM_DT_BF16 ? "bf16" : "f32", D, vec ? 1 : 0);
+  const dim3 blocks(static_cast<unsigned>(grid));
+  if (vec) hipLaunchKernelGGL((head_rows_kernel<A, D, MODE, true>), blocks, dim3(256), 0, s, p);
+  else hipLaunchKernelGGL((head_rows_kernel<A, D, MODE, false>), blocks, dim3(256), 0, s, p);
 }
 
 template <class A, int MODE>
@@ -392,12 +376,12 @@ am_status_code LaunchMode(const HeadRowArgs& p, bool vec, hipStream_t s) {
   const int64_t items = static_cast<int64_t>(p.rows) * (p.hq + p.hk + p.hv);
   if (items > kMaxItems) return SetLastError(AM_STATUS_INVALID_ARGUMENT, "head rows: too many rows");
   if (p.d == 64) {
-    LaunchHeadRowsD<A, MODE, 64>(p, vec, s);
+    LaunchHeadRows<A, MODE, 64>(p, vec, s);
   } else if (p.d == 128) {
-    LaunchHeadRowsD<A, MODE, 128>(p, vec, s);
+    LaunchHeadRows<A, MODE, 128>(p, vec, s);
   } else if constexpr (MODE != kAppendKv4) {
     if (p.d == 256) {
-      LaunchHeadRowsD<A, MODE, 256>(p, vec, s);
+      LaunchHeadRows<A, MODE, 256>(p, vec, s);
     } else {
       const int64_t grid = CeilDiv(items, 4);
       RecordLaunch(grid, 256, 0, "%s_any<%s,d=%d>", kModeName[MODE], A::kDtype == AM_DT_BF16 ? "bf16" : "f32", p.d);
@@ -419,34 +403,49 @@ struct ReadArgs {
   uint32_t seq, hkv, batch;
 };
 
-// A thread converts 8 values: 4 bytes of codes into 16 (bf16) or 32 (f32) bytes.  Threads
-// run over a row, then over the rows of one head, so the codes are read contiguously and
-// every row of the output is written in whole 128- or 256-byte pieces.  grid.y: k, v.
+// A thread converts 8 values of kReadRows rows: 4 bytes of codes into 16 (bf16) or 32 (f32)
+// bytes each.  A block's rows follow each other in one head's plane, so the codes are read
+// contiguously, and the output is written in whole rows of a head.  grid.y: k, v.  Four
+// sequences of 8192 rows (170 MB): 32.9 us, 5.2 TB/s, a copy's rate (one row a thread, its head
+// found by divisions, 42.8; four rows 33.0, eight 34.8; 37 rows 2.6, 2.9 and 3.0).
+constexpr int kReadRows = 2;
 template <class O, int D>
 __global__ __launch_bounds__(256) void kv4_read_kernel(ReadArgs p) {
-  constexpr uint32_t LP = D / 8;
-  const uint32_t i = blockIdx.x * (256 / LP) + threadIdx.x / LP;
+  constexpr uint32_t LP = D / 8, RB = 256 / LP;  // lanes of a row, rows of the block at a time
+  const uint32_t chunks = (p.seq + RB * kReadRows - 1) / (RB * kReadRows);
+  const uint32_t bg = blockIdx.x / chunks, first = (blockIdx.x - bg * chunks) * (RB * kReadRows) + threadIdx.x / LP;
+  const uint32_t b = bg / p.hkv, g = bg - b * p.hkv;
   const int sub = threadIdx.x % LP;
-  const uint32_t s = i % p.seq, bg = i / p.seq, g = bg % p.hkv, b = bg / p.hkv;
-  if (b >= p.batch || static_cast<int32_t>(s) >= live_rows(p.lens, b, static_cast<int32_t>(p.seq))) return;
-  const int64_t at = seq_position(p.start[b], s);
-  uint32_t w = 0, e = 0;
-  if (at >= 0 && at < p.cap) {
-    const int64_t row = p.kv.Row(b, g, at);
-    w = *reinterpret_cast<const uint32_t*>(p.codes[blockIdx.y] + row / 2 + 4 * sub);
-    e = p.scales[blockIdx.y][row / 32 + sub / 4];
-  }
-  uint32_t pair[4];
-  fp4_to_bf16(w, e8m0_scale_or_nan(e), pair);
-  const int64_t at_out = ((static_cast<int64_t>(b) * p.seq + s) * p.hkv + g) * D + 8 * sub;
-  if constexpr (O::kDtype == AM_DT_BF16) {
-    *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out[blockIdx.y]) + at_out) = make_uint4(pair[0], pair[1], pair[2], pair[3]);
-  } else {
-    float4* out = reinterpret_cast<float4*>(static_cast<float*>(p.out[blockIdx.y]) + at_out);
+  const uint32_t live = static_cast<uint32_t>(live_rows(p.lens, b, static_cast<int32_t>(p.seq)));
+  const int64_t start = seq_position(p.start[b], 0);
+  uint32_t w[kReadRows], e[kReadRows];
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
-      out[t] = make_float4(__uint_as_float(pair[2 * t] << 16), __uint_as_float(pair[2 * t] & 0xFFFF0000u),
-                           __uint_as_float(pair[2 * t + 1] << 16), __uint_as_float(pair[2 * t + 1] & 0xFFFF0000u));
+  for (int r = 0; r < kReadRows; ++r) {
+    const uint32_t s = first + r * RB;
+    const int64_t at = start + s;
+    w[r] = e[r] = 0;
+    if (s < live && at >= 0 && at < p.cap) {
+      const int64_t row = p.kv.Row(b, g, at);
+      w[r] = *reinterpret_cast<const uint32_t*>(p.codes[blockIdx.y] + row / 2 + 4 * sub);
+      e[r] = p.scales[blockIdx.y][row / 32 + sub / 4];
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < kReadRows; ++r) {
+    const uint32_t s = first + r * RB;
+    if (s >= live) return;
+    uint32_t pair[4];
+    fp4_to_bf16(w[r], e8m0_scale_or_nan(e[r]), pair);
+    const int64_t at_out = ((static_cast<int64_t>(b) * p.seq + s) * p.hkv + g) * D + 8 * sub;
+    if constexpr (O::kDtype == AM_DT_BF16) {
+      *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out[blockIdx.y]) + at_out) = make_uint4(pair[0], pair[1], pair[2], pair[3]);
+    } else {
+      float4* out = reinterpret_cast<float4*>(static_cast<float*>(p.out[blockIdx.y]) + at_out);
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+        out[t] = make_float4(__uint_as_float(pair[2 * t] << 16), __uint_as_float(pair[2 * t] & 0xFFFF0000u),
+                             __uint_as_float(pair[2 * t + 1] << 16), __uint_as_float(pair[2 * t + 1] & 0xFFFF0000u));
+    }
   }
 }
 
@@ -574,7 +573,7 @@ extern "C" am_status_code am_gfx950_kv4_read(const am_gfx950_kv4_read_args* a, v
   p.start = a->start_pos_dev, p.lens = a->seq_lens, p.cap = a->capacity;
   p.seq = static_cast<uint32_t>(a->seq), p.hkv = static_cast<uint32_t>(a->hkv), p.batch = static_cast<uint32_t>(a->batch);
   const int64_t lp = a->head_dim / 8;
-  const dim3 grid(static_cast<unsigned>(CeilDiv(a->batch * a->seq * a->hkv, 256 / lp)), 2);
+  const dim3 grid(static_cast<unsigned>(a->batch * a->hkv * CeilDiv(a->seq, 256 / lp * kReadRows)), 2);
   const bool bf = a->out_dtype == AM_DT_BF16;
   RecordLaunch(2 * static_cast<int64_t>(grid.x), 256, 0, "kv4_read<%s,d=%d>", bf ? "bf16" : "f32", static_cast<int>(a->head_dim));
   hipStream_t s = AsStream(stream);
