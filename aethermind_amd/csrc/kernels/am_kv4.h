@@ -42,7 +42,7 @@ inline bool Aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 
 // The stream belongs to the current device (whose CU count and kernels a call uses).
 am_status_code CheckStreamDevice(hipStream_t s);
 // Layout rules of AM_KV_MXFP4: head_dim, capacity, stride and alignment of the four caches.
-am_status_code CheckKv4Cache(const void* kc, const void* ks, const void* vc, const void* vs, int64_t batch, int64_t hkv,
+am_status_code CheckKv4Cache(const void* kc, const void* ks, const void* vc, const void* vs, int64_t batch,
                              int64_t head_dim, int64_t capacity, int64_t cbs, const am_gfx950_kv_pages* pages);
 
 }  // namespace am

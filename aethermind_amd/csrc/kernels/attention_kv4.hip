@@ -1127,7 +1127,9 @@ using namespace am;
 
 extern "C" int64_t am_gfx950_kv4_attention_workspace_bytes(int64_t batch, int64_t seq, int64_t hq, int64_t hkv,
                                                            int64_t head_dim, int64_t capacity) {
-  if (batch <= 0 || seq <= 0 || hkv <= 0 || hq <= 0 || capacity <= 0 || hq % hkv != 0 || hq / hkv > 16) return kTicketBytes;
+  if (batch <= 0 || seq <= 0 || hkv <= 0 || hq <= 0 || capacity <= 0 || hq % hkv != 0 || hq / hkv > 16 ||
+      batch > kMaxRows || seq > kMaxRows || hkv > 65536 || capacity >= (int64_t{1} << 31))
+    return kTicketBytes;  // no call takes these
   const int64_t G = hq / hkv, qt = std::min<int64_t>(16 / G, seq);
   return WorkspaceBytes(batch * CeilDiv(seq, qt), qt, G, hkv, head_dim, capacity);
 }
@@ -1140,12 +1142,12 @@ extern "C" am_status_code am_gfx950_kv4_attention(const am_gfx950_kv4_attention_
   AM_CHECK_ARG(a->batch >= 0 && a->seq >= 0 && a->capacity > 0 && a->capacity < (int64_t{1} << 31) - 64, "kv4_attention: bad shape");
   AM_CHECK_ARG(a->hkv <= 65536 && a->batch <= kMaxRows && a->seq <= kMaxRows && a->batch * a->seq <= kMaxRows,
                "kv4_attention: too many query rows");
-  AM_CHECK_ARG(std::isfinite(a->scale) && a->scale >= 0.0f, "kv4_attention: scale must be finite and not negative");
+  AM_CHECK_ARG(std::isfinite(a->scale * kLog2e) && a->scale >= 0.0f, "kv4_attention: scale must be finite and not negative");
   if (a->batch == 0 || a->seq == 0) return AM_STATUS_OK;
   AM_CHECK_ARG(a->q && a->out && a->start_pos_dev, "kv4_attention: null pointer");
   AM_CHECK_ARG(Aligned16(a->q) && Aligned16(a->out), "kv4_attention: q and out must be 16-byte aligned");
   const int64_t cbs = a->batch > 1 ? a->cache_batch_stride : 0;
-  if (auto st = CheckKv4Cache(a->k_codes, a->k_scales, a->v_codes, a->v_scales, a->batch, a->hkv, a->head_dim, a->capacity, cbs, a->pages);
+  if (auto st = CheckKv4Cache(a->k_codes, a->k_scales, a->v_codes, a->v_scales, a->batch, a->head_dim, a->capacity, cbs, a->pages);
       st != AM_STATUS_OK)
     return st;
   Attn4Args p{};

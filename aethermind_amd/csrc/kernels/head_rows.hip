@@ -18,7 +18,7 @@ am_status_code CheckStreamDevice(hipStream_t s) {
   return AM_STATUS_OK;
 }
 
-am_status_code CheckKv4Cache(const void* kc, const void* ks, const void* vc, const void* vs, int64_t batch, int64_t hkv,
+am_status_code CheckKv4Cache(const void* kc, const void* ks, const void* vc, const void* vs, int64_t batch,
                              int64_t head_dim, int64_t capacity, int64_t cbs, const am_gfx950_kv_pages* pages) {
   AM_CHECK_ARG(head_dim == 64 || head_dim == 128, "kv4 cache: head_dim must be 64 or 128");
   AM_CHECK_ARG(kc && ks && vc && vs, "kv4 cache: null code or scale cache");
@@ -30,7 +30,6 @@ am_status_code CheckKv4Cache(const void* kc, const void* ks, const void* vc, con
       AM_CHECK_ARG(cbs >= 0 && cbs % (32 * head_dim) == 0,
                    "kv4 cache: cache_batch_stride must be a multiple of 32 * head_dim values");
   }
-  (void)hkv;
   return AM_STATUS_OK;
 }
 
@@ -358,7 +357,7 @@ __global__ __launch_bounds__(256) void head_rows_any_kernel(HeadRowArgs p) {
   }
 }
 
-constexpr int64_t kMaxItems = int64_t{1} << 26;  // head rows of a call (a grid has at most 2^32 threads)
+constexpr int64_t kMaxItems = int64_t{1} << 25;  // head rows of a call (a grid has fewer than 2^32 threads)
 
 const char* const kModeName[] = {"qk_norm_rope", "kv_append", "kv_append_kv4"};
 
@@ -523,7 +522,7 @@ extern "C" am_status_code am_gfx950_kv_append(const am_gfx950_kv_append_args* a,
   const bool four = a->cache_format == AM_KV_MXFP4;
   const int64_t cbs = a->batch > 1 ? a->cache_batch_stride : 0;
   if (four)
-    if (auto st = CheckKv4Cache(a->k_cache, a->k_scales, a->v_cache, a->v_scales, a->batch, a->hkv, d, a->capacity, cbs, a->pages);
+    if (auto st = CheckKv4Cache(a->k_cache, a->k_scales, a->v_cache, a->v_scales, a->batch, d, a->capacity, cbs, a->pages);
         st != AM_STATUS_OK)
       return st;
   HeadRowArgs p{};
@@ -562,7 +561,7 @@ extern "C" am_status_code am_gfx950_kv4_read(const am_gfx950_kv4_read_args* a, v
   AM_CHECK_ARG(a->k_out && a->v_out && a->start_pos_dev, "kv4_read: null pointer");
   AM_CHECK_ARG(Aligned16(a->k_out) && Aligned16(a->v_out), "kv4_read: outputs must be 16-byte aligned");
   const int64_t cbs = a->batch > 1 ? a->cache_batch_stride : 0;
-  if (auto st = CheckKv4Cache(a->k_codes, a->k_scales, a->v_codes, a->v_scales, a->batch, a->hkv, a->head_dim, a->capacity, cbs, a->pages);
+  if (auto st = CheckKv4Cache(a->k_codes, a->k_scales, a->v_codes, a->v_scales, a->batch, a->head_dim, a->capacity, cbs, a->pages);
       st != AM_STATUS_OK)
     return st;
   ReadArgs p{};
@@ -573,7 +572,9 @@ extern "C" am_status_code am_gfx950_kv4_read(const am_gfx950_kv4_read_args* a, v
   p.start = a->start_pos_dev, p.lens = a->seq_lens, p.cap = a->capacity;
   p.seq = static_cast<uint32_t>(a->seq), p.hkv = static_cast<uint32_t>(a->hkv), p.batch = static_cast<uint32_t>(a->batch);
   const int64_t lp = a->head_dim / 8;
-  const dim3 grid(static_cast<unsigned>(a->batch * a->hkv * CeilDiv(a->seq, 256 / lp * kReadRows)), 2);
+  const int64_t blocks = a->batch * a->hkv * CeilDiv(a->seq, 256 / lp * kReadRows);
+  AM_CHECK_ARG(blocks < (int64_t{1} << 23), "kv4_read: too many rows");
+  const dim3 grid(static_cast<unsigned>(blocks), 2);
   const bool bf = a->out_dtype == AM_DT_BF16;
   RecordLaunch(2 * static_cast<int64_t>(grid.x), 256, 0, "kv4_read<%s,d=%d>", bf ? "bf16" : "f32", static_cast<int>(a->head_dim));
   hipStream_t s = AsStream(stream);

@@ -410,15 +410,18 @@ am_status_code am_gfx950_kv4_read(const am_gfx950_kv4_read_args* args, void* hip
  * one past the cache has all of them.  Rows behind seq_lens[b] are left as they were.
  * out = sum_t softmax_t(scale * q . K_t) V_t over the values that the cache stands for;
  * q head h reads kv head h / (hq / hkv), at most 16 q heads per kv head and 65535 query
- * rows; fp32 online softmax; the products take q as it is (bf16) or as three bf16 parts (fp32) and the
- * probabilities as two or three, so neither adds to the one rounding of out.  Scores of
- * which none exceeds minus infinity give zeros.  A NaN among a row's keys gives NaN (a NaN
- * value only in its own 32 dimensions); what the cache holds past a row's keys does not
- * matter.  q and out are 16-byte aligned.
+ * rows; fp32 online softmax and sums.  The products take q as it is (bf16) or as three bf16
+ * parts (fp32), and the probabilities as two or three; bf16 calls of many rows round the
+ * probabilities to f16 instead (11 bits where out has 8) and hold a value to 2^-38 of the
+ * largest of its head's 32 dimensions among the keys.
+ * Scores of which none exceeds minus infinity give zeros.  A NaN among a row's keys gives
+ * NaN (a NaN value only in its own 32 dimensions); what the cache holds past a row's keys
+ * does not matter.  q and out are 16-byte aligned.
  * workspace: am_gfx950_kv4_attention_workspace_bytes(...) bytes, 16-byte aligned, whose
  * first 16384 bytes must be zero before the first call and are left zero.  One workspace
- * serves calls of any shapes in turn; calls that overlap on one workspace race.  The
- * results do not depend on the scheduling of blocks. */
+ * serves this function's calls of any shapes in turn (not am_gfx950_attention's, whose
+ * records would reach into those bytes); calls that overlap on one workspace race.  Equal
+ * calls give equal bits. */
 typedef struct am_gfx950_kv4_attention_args {
   const void* q;
   void* out;

@@ -239,6 +239,24 @@ def test_append_kv4(dtype, d, hq, hkv, block, b, n, start, lens, gains):
             check_rows(q_out.view(-1, hq, d)[rows], q.reshape(-1, hq, d)[rows], qw, 1e-5, cos, sin, pos[rows], dtype, "q_out")
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("d", [64, 128])
+def test_append_kv4_unaligned_inputs(dtype, d):
+    """inputs that are not vector-aligned give the codes of aligned ones"""
+    g, b, n, hq, hkv, cap = gen_of(d), 2, 9, 3, 2, 64
+    wide = randn(g, b * n, (hq + 2 * hkv) * d + 1).to(DTYPES[dtype][0])
+    w = (1 + randn(g, d + 1) / 4).to(DTYPES[dtype][0])
+    cos, sin = R.tables(cap, d)
+    got = []
+    for x, gain in ((wide[:, 1:], w[1:]), (wide[:, 1:].contiguous(), w[1:].clone())):
+        c = Cache(b, hkv, cap, d)
+        q_out = torch.zeros(b * n, hq * d, dtype=wide.dtype, device="cuda")
+        R.append(c, x[:, : hq * d], x[:, hq * d : (hq + hkv) * d], x[:, (hq + hkv) * d :], q_out, b, n, hq, i64(3, 40), q_w=gain, k_w=gain,
+                 cos=cos, sin=sin, dtype=dtype)
+        got.append((q_out, *c.t.values()))
+    assert all(torch.equal(x, y) for x, y in zip(*got))
+
+
 def test_append_kv4_unassigned_blocks():
     """table entries outside the pool: those rows are not written and the pages' flag is set"""
     g, b, n, hkv, d, cap = gen_of(2), 1, 96, 2, 64, 128
@@ -395,6 +413,12 @@ def test_attention_decode(dtype, block, ctx):
     attention_case(len(ctx), len(ctx), 1, 32, 8, 128, 2080, [t - 1 for t in ctx], block=block, dtype=dtype)
 
 
+@pytest.mark.parametrize("n", [1, 3, 400])
+def test_attention_paged_capacity_inside_a_block(n):
+    """a capacity that ends inside a block, and inside a step of 32 keys: rows at and past it"""
+    attention_case(n, 1, n, 64, 16, 64, 405, [404 - n // 2], block=64, behind="nan" if n == 1 else "")
+
+
 def test_attention_one_long_row():
     attention_case(1, 1, 1, 8, 2, 128, 20000 - 20000 % 32, [19900])
 
@@ -497,6 +521,7 @@ def test_attention_shared_prefix_stride_zero():
     (64, 64, 128, 1, 300, [-30], None, 0),              # rows before position 0
     (64, 64, 64, 1, 300, [20], None, 0),                # past the cache
     (256, 16, 64, 1, 100, [0], None, 0),                # sixteen heads a group
+    (64, 16, 64, 1, 400, [2300], None, 32),             # more blocks than a wave holds of the table
     (32, 8, 128, 16, 33, [31 * i for i in range(16)], [33 - 2 * i for i in range(16)], 32),  # a second block of one row
 ])
 def test_attention_many_rows(dtype, hq, hkv, d, b, n, start, lens, block):

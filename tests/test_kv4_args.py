@@ -73,12 +73,13 @@ BAD = {
         dict(out_dtype=N.AM_DT_I32), dict(batch=-1), dict(seq=-1), dict(hkv=0), dict(capacity=0), dict(capacity=48),
         dict(head_dim=96), dict(head_dim=256), dict(k_codes=None), dict(k_scales=None), dict(v_codes=None), dict(v_scales=None),
         dict(k_out=None), dict(v_out=None), dict(k_out=P + 2), dict(start_pos_dev=None), dict(k_codes=P + 1),
-        dict(cache_batch_stride=100), dict(batch=1 << 60, seq=16), dict(seq=1 << 27), dict(pages=pages(table_stride=1))]),
+        dict(cache_batch_stride=100), dict(batch=1 << 60, seq=16), dict(seq=1 << 27),
+        dict(batch=1 << 24, seq=1, hkv=1, cache_batch_stride=64 * 64), dict(pages=pages(table_stride=1))]),
     "am_gfx950_kv4_attention": (attention_args, [
         dict(dtype=N.AM_DT_F16), dict(hq=0), dict(hkv=0), dict(hq=7), dict(hq=34), dict(batch=-1), dict(seq=-1), dict(capacity=0),
         dict(capacity=1 << 31), dict(capacity=40), dict(head_dim=96), dict(head_dim=32), dict(q=None), dict(out=None),
         dict(q=P + 2), dict(out=P + 8), dict(k_codes=None), dict(v_scales=None), dict(k_scales=P + 2), dict(start_pos_dev=None),
-        dict(scale=-1.0), dict(scale=NAN), dict(scale=INF), dict(workspace=None), dict(workspace=P + 4), dict(workspace_bytes=0),
+        dict(scale=-1.0), dict(scale=NAN), dict(scale=INF), dict(scale=3e38), dict(workspace=None), dict(workspace=P + 4), dict(workspace_bytes=0),
         dict(workspace_bytes=16384), dict(cache_batch_stride=33 * 64), dict(cache_batch_stride=-8192), dict(batch=1 << 17),
         dict(seq=1 << 25), dict(pages=pages(block_size=24)), dict(pages=pages(table_stride=1))]),
 }
@@ -107,7 +108,7 @@ def test_workspace_bytes():
     """never below the tickets; a workspace of a call's own size is accepted up to its last byte's check"""
     f = N.lib().am_gfx950_kv4_attention_workspace_bytes
     for bad in ((0, 1, 8, 2, 64, 64), (1, 0, 8, 2, 64, 64), (1, 1, 7, 2, 64, 64), (1, 1, 64, 2, 64, 64), (1, 1, 8, 0, 64, 64),
-                (1, 1, 8, 2, 64, 0)):
+                (1, 1, 8, 2, 64, 0), (1 << 62, 1, 8, 2, 64, 64), (1, 1 << 62, 8, 2, 64, 64), (1, 1, 8, 2, 64, 1 << 62)):
         assert f(*bad) == 16384
     for shape in ((1, 1, 32, 8, 128, 131072), (16, 1, 32, 8, 128, 8192), (1, 1, 16, 1, 128, 1 << 20), (300, 1, 8, 2, 64, 4096),
                   (1, 37, 32, 8, 128, 1024), (1, 2048, 32, 8, 128, 8192)):
