@@ -568,10 +568,13 @@ __global__ __launch_bounds__(NW * 64, F32 ? 2 : 4) void kv4_attention_kernel(Att
 //     ds_read_b64_tr_b16.
 //   * bf16 q: P is f16, 11 bits where bf16 has 8 (its rounding is 1/8 of out's own), in one
 //     product instead of the two of a bf16 split.  V is f16 as well: codes times 2^(e - E) with E
-//     the largest scale of the group's 32 dimensions among the block's keys, less 13, and exact
-//     to 2^-36 of that largest one; the block reads its keys' scale bytes once beforehand (1/17 of
-//     the cache).  P carries 2^14 so that its small values stay normal.  Row sums are those of
-//     the rounded P.  fp32 q: three bf16 parts of q and P, bf16 V.
+//     the largest scale of the group's 32 dimensions among the block's keys, less 13; the block
+//     reads its keys' scale bytes once beforehand (1/17 of the cache).  P carries 2^14 so that its
+//     small values stay normal (below 2^-28 they are held to 2^-39).  Row sums are those of the
+//     rounded P.  Where a group's scales differ by more than 2^16, a value that one row alone sees
+//     could push another row's out of f16: such a block takes bf16 V and P in two bf16 parts (2048
+//     rows at 6144 keys: 386 us for 300).
+//   * fp32 q: three bf16 parts of q and P, bf16 V.
 //   * The same pass over the scales finds the first NaN value of each group; it enters the
 //     products as zero and spoils the columns that see its key at the end.
 // What bounds it: VALU work (a tile costs a wave about 120 instructions, 57 of them the
@@ -583,10 +586,18 @@ typedef __attribute__((ext_vector_type(4))) short s16x4_t;
 typedef __attribute__((ext_vector_type(2))) unsigned short u16x2_t;
 constexpr int kWideWaves = 4;   // waves of columns of a block
 constexpr int kVTop = 140;      // exponent byte of the largest scale of V in f16: 6 * 2^13
+constexpr int kNear = 17;        // f16: the largest scale byte of a group less (the smallest - 1)
 constexpr float kPBias = 14.0f;  // log2 of the factor on P in f16
 
 __device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
   return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2_t, a), __builtin_bit_cast(u16x2_t, b)));
+}
+
+__device__ __forceinline__ uint32_t min_u16x2(uint32_t a, uint32_t b) {
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_min(__builtin_bit_cast(u16x2_t, a), __builtin_bit_cast(u16x2_t, b)));
+}
+__device__ __forceinline__ uint32_t less_one_u16x2(uint32_t a) {
+  return __builtin_bit_cast(uint32_t, static_cast<u16x2_t>(__builtin_bit_cast(u16x2_t, a) - u16x2_t{1, 1}));
 }
 
 // Slot of a tile's row (D values, SL slots of 16 bytes) that holds slot s of key `key`: the 16
@@ -645,7 +656,7 @@ __global__ __launch_bounds__(512) void kv4_attention_wide_kernel(Attn4Args p) {
   constexpr int NT = QW * KS * 64, GT = QW * 64;      // threads of the block, of a key group
   constexpr int PC = kStep * SL;                      // pieces (8 values) of a tile of K, of V
   constexpr int NP = 2 * PC / GT;                     // pieces of a thread per tile
-  constexpr int QP = F32 ? 3 : 1;
+  constexpr int QP = F32 ? 3 : 1;                     // bf16 parts of q
   constexpr int DT = D / 32;
   constexpr int OW = DT * 16 + 2;                     // words of a lane's state
   static_assert(PC % GT == 0 && GT % SL == 0, "a thread's pieces are K or V by their number alone");
@@ -654,7 +665,7 @@ __global__ __launch_bounds__(512) void kv4_attention_wide_kernel(Attn4Args p) {
   constexpr int kSmem = std::max(KS * NB * 2 * kTileBytes, (KS - 1) * QW * OW * 256);
   static_assert(NT == 512, "two waves per SIMD, one of each half");
   __shared__ __align__(16) uint8_t smem_w[kSmem];     // per key group and buffer: K, V
-  __shared__ uint32_t s_top[GR];                      // largest scale of V
+  __shared__ uint32_t s_top[GR], s_low[GR];           // largest and smallest scale of V
   __shared__ int32_t s_nan[GR];                       // first key with a NaN value
 
   const int kg = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / GT);
@@ -745,9 +756,11 @@ __global__ __launch_bounds__(512) void kv4_attention_wide_kernel(Attn4Args p) {
     next_off = tile_off(kg + KS);
   }
 
-  // the block's scales of V: the largest and the first NaN of each group
+  // the block's scales of V: the largest, the smallest (but for 0, the scale of zeros) and the first
+  // NaN of each group
   if (threadIdx.x < GR) {
     s_top[threadIdx.x] = 0;
+    s_low[threadIdx.x] = 0xFFFF;
     s_nan[threadIdx.x] = 0x7FFFFFFF;
   }
   __syncthreads();
@@ -766,26 +779,35 @@ __global__ __launch_bounds__(512) void kv4_attention_wide_kernel(Attn4Args p) {
         }
       }
     };
-    uint32_t even = 0, odd = 0;  // two bytes of each word as 16-bit values
+    // two bytes of each word as 16-bit values; the smallest less one, so that 0 is no value
+    uint32_t top[2] = {0, 0}, low[2] = {~0u, ~0u};
     scan([&](uint32_t w, int) {
-      even = max_u16x2(even, w & 0x00FF00FFu);
-      odd = max_u16x2(odd, (w >> 8) & 0x00FF00FFu);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const uint32_t x = (w >> (8 * i)) & 0x00FF00FFu;
+        top[i] = max_u16x2(top[i], x);
+        low[i] = min_u16x2(low[i], less_one_u16x2(x));
+      }
     });
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-      even = max_u16x2(even, static_cast<uint32_t>(__shfl_xor(static_cast<int>(even), o)));
-      odd = max_u16x2(odd, static_cast<uint32_t>(__shfl_xor(static_cast<int>(odd), o)));
-    }
-    if (lane == 0) {
-      const uint32_t m[4] = {even & 0xFFFFu, odd & 0xFFFFu, even >> 16, odd >> 16};
+    for (int i = 0; i < 2; ++i)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) atomicMax(&s_top[e % GR], m[e]);
+      for (int o = 32; o > 0; o >>= 1) {
+        top[i] = max_u16x2(top[i], static_cast<uint32_t>(__shfl_xor(static_cast<int>(top[i]), o)));
+        low[i] = min_u16x2(low[i], static_cast<uint32_t>(__shfl_xor(static_cast<int>(low[i]), o)));
+      }
+    if (lane == 0) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        atomicMax(&s_top[e % GR], (top[e & 1] >> (8 * (e & 2))) & 0xFFFFu);
+        atomicMin(&s_low[e % GR], (low[e & 1] >> (8 * (e & 2))) & 0xFFFFu);
+      }
     }
     __syncthreads();
     uint32_t any = 0;
 #pragma unroll
     for (int e = 0; e < GR; ++e) any = max(any, s_top[e]);
-    if (any >= kScaleNan) {  // again, byte by byte (block-uniform)
+    if (any >= kScaleNan) {  // the largest again, byte by byte (block-uniform)
       __syncthreads();
       if (threadIdx.x < GR) s_top[threadIdx.x] = 0;
       __syncthreads();
@@ -799,6 +821,13 @@ __global__ __launch_bounds__(512) void kv4_attention_wide_kernel(Attn4Args p) {
       __syncthreads();
     }
   }
+  bool near = true;  // (block-uniform) the groups' scales lie close enough for f16
+#pragma unroll
+  for (int e = 0; e < GR; ++e) near = near && static_cast<int>(s_top[e]) - static_cast<int>(s_low[e]) <= kNear;
+
+  // The walk over the keys.  H: V and P in f16.
+  auto run = [&]<bool H>() {
+  constexpr int PP = H ? 1 : F32 ? 3 : 2;  // parts of P
 
   // (buffer of the group's u-th tile)
   auto tile_k = [&](int u) { return smem_w + (kg * NB + (u & (NB - 1))) * 2 * kTileBytes; };
@@ -816,7 +845,7 @@ __global__ __launch_bounds__(512) void kv4_attention_wide_kernel(Attn4Args p) {
         *reinterpret_cast<uint4*>(tile_k(u) + key * (2 * D) + 16 * k_slot<SL>(key, psl)) = make_uint4(w[0], w[1], w[2], w[3]);
       } else {
         const bool dead = (sb >= kScaleNan) | (kStep * t + key >= kend);
-        if constexpr (F32) {
+        if constexpr (!H) {
           fp4_to_bf16(code[c], e8m0_scale(dead ? 0u : sb), w);
         } else {
           const float s = e8m0_scale(static_cast<uint32_t>(max(static_cast<int>(dead ? 0u : sb) + (dead ? 0 : v_add), 0)));
@@ -838,7 +867,7 @@ __global__ __launch_bounds__(512) void kv4_attention_wide_kernel(Attn4Args p) {
     for (int r = 0; r < 16; ++r) o[dt][r] = 0.0f;
 
   f32x16_t acc;                                  // scores
-  uint32_t pw[F32 ? 3 : 1][2][4];                // P operand: parts, chunks of 16 keys
+  uint32_t pw[PP][2][4];                         // P operand: parts, chunks of 16 keys
   auto softmax = [&](int u) {
     const int t = u * KS + kg;
     if (kStep * t + kStep > least) {  // some column of the wave ends in or before this tile
@@ -863,16 +892,16 @@ __global__ __launch_bounds__(512) void kv4_attention_wide_kernel(Attn4Args p) {
         for (int r = 0; r < 16; ++r) o[dt][r] *= cf;
       m_run = mn;
     }
-    const float sub = (F32 ? 0.0f : kPBias) - (m_run == -INFINITY ? 0.0f : m_run);
+    const float sub = (H ? kPBias : 0.0f) - (m_run == -INFINITY ? 0.0f : m_run);
 #pragma unroll
     for (int r = 0; r < 16; r += 2) {
       float v0 = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[r], p.scale, sub));
       float v1 = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[r + 1], p.scale, sub));
-      if constexpr (F32) {
+      if constexpr (!H) {
         l_run += v0;
         l_run += v1;
 #pragma unroll
-        for (int i = 0; i < 3; ++i) {
+        for (int i = 0; i < PP; ++i) {
           const uint32_t w = __builtin_bit_cast(uint32_t, bf16x2_t{static_cast<__bf16>(v0), static_cast<__bf16>(v1)});
           pw[i][r / 8][(r % 8) / 2] = w;
           v0 -= __uint_as_float(w << 16);
@@ -903,9 +932,9 @@ __global__ __launch_bounds__(512) void kv4_attention_wide_kernel(Attn4Args p) {
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) {
       const auto a = __builtin_shufflevector(part[dt][0], part[dt][1], 0, 1, 2, 3, 4, 5, 6, 7);
-      if constexpr (F32) {
+      if constexpr (!H) {
 #pragma unroll
-        for (int i = 2; i >= 0; --i)
+        for (int i = PP - 1; i >= 0; --i)
           o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
               __builtin_bit_cast(bf16x8_t, a),
               __builtin_bit_cast(bf16x8_t, make_uint4(pw[i][c][0], pw[i][c][1], pw[i][c][2], pw[i][c][3])), o[dt], 0, 0, 0);
@@ -924,11 +953,11 @@ __global__ __launch_bounds__(512) void kv4_attention_wide_kernel(Attn4Args p) {
     for (int i = QP - 1; i >= 0; --i) acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k, qop[i][kk], acc, 0, 0, 0);
   };
   // M of tile u: P V of tile u - 1 and K Q^T of tile u.  Its operands are read ahead, so that
-  // the products do not wait for LDS (fp32 q leaves no registers for that: read_m does nothing).
-  s16x4_t vop[F32 ? 1 : 2][DT][2];
-  bf16x8_t kop[F32 ? 1 : D / 16];
+  // the products do not wait for LDS (without H there are no registers for that: read_m does nothing).
+  s16x4_t vop[H ? 2 : 1][DT][2];
+  bf16x8_t kop[H ? D / 16 : 1];
   auto read_m = [&](int u, bool pv, bool qk) {
-    if constexpr (!F32) {
+    if constexpr (H) {
       if (pv) {
         read_v(u - 1, 0, vop[0]);
         read_v(u - 1, 1, vop[1]);
@@ -943,8 +972,8 @@ __global__ __launch_bounds__(512) void kv4_attention_wide_kernel(Attn4Args p) {
     if (pv) {
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        if constexpr (F32) read_v(u - 1, c, vop[0]);
-        products(c, vop[F32 ? 0 : c]);
+        if constexpr (!H) read_v(u - 1, c, vop[0]);
+        products(c, vop[H ? c : 0]);
       }
     }
     if (qk) {
@@ -952,8 +981,8 @@ __global__ __launch_bounds__(512) void kv4_attention_wide_kernel(Attn4Args p) {
       for (int r = 0; r < 16; ++r) acc[r] = 0.0f;
 #pragma unroll
       for (int kk = 0; kk < D / 16; ++kk) {
-        if constexpr (F32) score(kk, read_k(u, kk));
-        else score(kk, kop[kk]);
+        if constexpr (H) score(kk, kop[kk]);
+        else score(kk, read_k(u, kk));
       }
     }
   };
@@ -962,7 +991,7 @@ __global__ __launch_bounds__(512) void kv4_attention_wide_kernel(Attn4Args p) {
   // of the staging) and products (M: P V of tile u, K Q^T of tile u + 1).  Between two barriers
   // the first group does V then M, and the second, which shares every SIMD with it, M (of the
   // tile before) then V: while one wave of a SIMD multiplies the other exponentiates.  In phase
-  // (every wave V then M, a barrier a tile) 2048 rows at 6144 keys took 329 us, so 294.
+  // (every wave V then M, a barrier a tile) 2048 rows at 6144 keys took 329 us, so 300.
   // Interval u stores tile u + 2.  K of tile x is read in interval x - 1 (ahead of x in the
   // second group), its V in x or x + 1: four buffers.
   // (kg as a lane value: as a scalar one the loops' registers spill)
@@ -1056,7 +1085,7 @@ __global__ __launch_bounds__(512) void kv4_attention_wide_kernel(Attn4Args p) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         v[e] = o[dt][4 * r4 + e] * inv;
-        if constexpr (!F32) v[e] = __builtin_ldexpf(v[e], back);
+        if constexpr (H) v[e] = __builtin_ldexpf(v[e], back);
         if (bad) v[e] = __builtin_nanf("");
       }
       const int64_t to = qrow + 32 * dt + 8 * r4 + 4 * h;
@@ -1068,6 +1097,13 @@ __global__ __launch_bounds__(512) void kv4_attention_wide_kernel(Attn4Args p) {
         *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + to) = make_uint2(w0, w1);
       }
     }
+  }
+  };
+  if constexpr (F32) {
+    run.template operator()<false>();
+  } else {
+    if (near) run.template operator()<true>();
+    else run.template operator()<false>();
   }
 }
 

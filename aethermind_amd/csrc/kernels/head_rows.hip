@@ -13,7 +13,8 @@ namespace am {
 am_status_code CheckStreamDevice(hipStream_t s) {
   if (s == nullptr) return AM_STATUS_OK;
   int cur = -1, sdev = -1;
-  if (hipGetDevice(&cur) != hipSuccess || hipStreamGetDevice(s, &sdev) != hipSuccess || cur != sdev)
+  if (hipGetDevice(&cur) != hipSuccess || hipStreamGetDevice(s, &sdev) != hipSuccess) (void)hipGetLastError();  // (else the next launch's)
+  if (cur < 0 || cur != sdev)
     return SetLastError(AM_STATUS_INVALID_ARGUMENT, "the stream's device is not the current device");
   return AM_STATUS_OK;
 }

@@ -550,6 +550,28 @@ def test_attention_many_rows_spread_values(dtype):
     assert ((out.double().view_as(want) - want).abs() <= R.attention_bound(want, mag, top, cap, d, dtype)).all()
 
 
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("up", [0, 8, 16, 17, 18, 40, 120])
+def test_attention_many_rows_distant_later_values(d, up):
+    """a later key's value of 2^up times the others', inside the rows of one block: the rows before it do not notice"""
+    g, n, hq, hkv, cap, b = gen_of(d), 400, 64, 16, 416, 1
+    c = Cache(1, hkv, cap, d)
+    k, v = randn(g, 1, hkv, cap, d), randn(g, 1, hkv, cap, d) * 2.0**-50
+    v[:, :, 77] *= 2.0**up
+    v[:, :, 251, :32] = 0
+    c.put_values("k", k)
+    c.put_values("v", v)
+    q = randn(g, n, hq * d).to(torch.bfloat16)
+    out, ws = torch.empty_like(q), R.workspace(1, n, hq, hkv, d, cap)
+    R.attend(c, q, out, 1, n, hq, i64(0), ws)
+    assert N.last_launch().kernel.startswith(b"kv4_attention_wide")
+    want, mag, top = R.attention(q.double().view(1, n, hq, d), c.values("k"), c.values("v"), [0], [n], R.softmax_scale(d))
+    got = out.double().view_as(want)
+    assert (got.abs().amax((0, 2, 3)) > 0).all()
+    # attention_bound with its floor (1e-30) scaled as the values are
+    assert ((got - want).abs() * 2.0**50 <= R.attention_bound(want * 2.0**50, mag * 2.0**50, top, cap, d, "bf16")).all()
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 @pytest.mark.parametrize("d", [64, 128])
 def test_attention_many_rows_nan(dtype, d):
@@ -573,6 +595,58 @@ def test_attention_many_rows_nan(dtype, d):
         got = out.view(n, hq, d)
         assert torch.equal(torch.isnan(got), bad)
         assert (((got.double() - want[0]).abs() <= R.attention_bound(want, mag, top, cap, d, dtype)[0]) | bad).all()
+
+
+@pytest.mark.parametrize("block", [0, 4096])
+def test_offsets_past_32_bits(block):
+    """caches of 2^34 values: rows written, read and attended to where offsets in values (and in bytes) pass 2^32; scores of
+    the rows before them are 0 beside ones near 60, values 0, so that they add nothing"""
+    g, b, hq, hkv, d, cap, n = gen_of(4), 2, 8, 2, 128, 2**25 + 96, 40
+    c = Cache(b, hkv, cap, d, block, fill=0, scale_fill=0)
+    start = [cap - n, cap - 4000]
+    kv = randn(g, b * n, 2 * hkv * d).to(torch.bfloat16)
+    code, scale = R.encode(kv.view(b, n, 2, hkv, d))
+    cos, sin = torch.ones(cap, d // 2, device="cuda"), torch.zeros(cap, d // 2, device="cuda")
+    R.append(c, None, kv[:, : hkv * d], kv[:, hkv * d :], None, b, n, 0, i64(*start), cos=cos, sin=sin)
+    del cos, sin
+    for i in range(b):
+        for m, t in (("k", 0), ("v", 1)):
+            for r in (0, n - 1):
+                at = start[i] + r
+                row = c.t[m][i, :, at] if not block else c.t[m][int(c.table[i, at // block]), :, at % block]
+                assert torch.equal(row, R.pack(code[i, r, t])), (m, i, r)
+    k, v = R.read(c, b, n, i64(*start))
+    values = R.decode(R.pack(code), scale)  # [b][n][2][hkv][d]
+    assert torch.equal(k.double().view(b, n, hkv, d), values[:, :, 0]) and torch.equal(v.double().view(b, n, hkv, d), values[:, :, 1])
+    # a row at the end of each sequence's keys: q along its first key, 60 in the exponent
+    q = torch.empty(b, hq, d, device="cuda")
+    for h in range(hq):
+        key = values[:, 0, 0, h // (hq // hkv)].float()
+        q[:, h] = key * (60 * d**0.5 / key.square().sum(-1, keepdim=True))
+    q = q.to(torch.bfloat16)
+    out, at = torch.empty(b, hq, d, dtype=torch.bfloat16, device="cuda"), i64(*[s + n - 1 for s in start])
+    R.attend(c, q, out, b, 1, hq, at, R.workspace(b, 1, hq, hkv, d, cap))
+    planes = values.permute(2, 0, 3, 1, 4)  # [2][b][hkv][n][d]
+    want, mag, top = R.attention(q.double().view(b, 1, hq, d), planes[0], planes[1], [n - 1] * b, [1] * b, R.softmax_scale(d))
+    # the other keys' share: 2^26 e^-60 < 2^-60
+    assert ((out.double().view_as(want) - want).abs() <= R.attention_bound(want, mag, top, 2 * n, d, "bf16")).all()
+    # the kernel of many rows, at the front of each sequence's planes (the second head's start past 2^32)
+    c.t["k"].zero_(), c.t["v"].zero_()
+    m, hd = 1024, 64
+    kv = randn(g, b * m, 2 * hkv * d).to(torch.bfloat16)
+    cos, sin = torch.ones(cap, hd, device="cuda"), torch.zeros(cap, hd, device="cuda")
+    R.append(c, None, kv[:, : hkv * d], kv[:, hkv * d :], None, b, m, 0, i64(0, 0), cos=cos, sin=sin)
+    q = randn(g, b * m, hq * d).to(torch.bfloat16)
+    out = torch.empty_like(q)
+    R.attend(c, q, out, b, m, hq, i64(0, 0), R.workspace(b, m, hq, hkv, d, cap))
+    assert N.last_launch().kernel.startswith(b"kv4_attention_wide")
+    code, scale = R.encode(kv.view(b, m, 2, hkv, d))
+    planes = R.decode(R.pack(code), scale).permute(2, 0, 3, 1, 4)
+    rows = [0, 31, 500, m - 1]
+    for r in rows:
+        want, mag, top = R.attention(q.double().view(b, m, hq, d)[:, r : r + 1], planes[0], planes[1], [r] * b, [1] * b, R.softmax_scale(d))
+        got = out.double().view(b, m, hq, d)[:, r : r + 1]
+        assert ((got - want).abs() <= R.attention_bound(want, mag, top, m, d, "bf16")).all()
 
 
 # ------------------------------------------------------------------ together
@@ -686,3 +760,29 @@ def test_other_stream():
         m.step(ws)
     torch.cuda.current_stream().wait_stream(side)
     assert torch.equal(m.out, want)
+
+
+def test_two_streams_at_once():
+    """calls that overlap, each with a workspace and a cache of its own, give what they give alone"""
+    g, models, alone = gen_of(14), [Model(2, 32, 8, 128, 16384, 64), Model(1, 16, 4, 128, 32768, 0)], []
+    spaces = [R.workspace(m.b, 1, m.hq, m.c.hkv, m.c.d, m.c.cap) for m in models]
+    for m, ws in zip(models, spaces):
+        for n in ("k", "v"):
+            m.c.put_values(n, randn(g, m.b, m.c.hkv, m.c.cap, m.c.d))
+        m.qkv.copy_(randn(g, *m.qkv.shape))
+        m.start.copy_(torch.arange(m.b, device="cuda") * 500 + 15000)
+        m.step(ws)
+        alone.append(m.out.clone())
+        m.out.zero_()
+    streams = [torch.cuda.Stream() for _ in models]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(20):
+        for m, ws, s in zip(models, spaces, streams):
+            with torch.cuda.stream(s):
+                m.step(ws)
+    for s in streams:
+        torch.cuda.current_stream().wait_stream(s)
+    for m, ws, want in zip(models, spaces, alone):
+        assert torch.equal(m.out, want)
+        assert not ws[:16384].any()
