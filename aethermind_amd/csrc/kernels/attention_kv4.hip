@@ -164,6 +164,45 @@ __device__ __forceinline__ void lds_barrier() {
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
+// Row offsets, in elements, of the steps first, first + every, ... (up to last) of (b, g): KvRows::Row
+// of a step's first key without a table read in front of its loads.  A lane holds the block-table
+// entry of one of 64 visits; planes are one block without end.
+struct StepWalk {
+  const int32_t* table;
+  int64_t block_elems, base;
+  int32_t num_blocks, stride, shift, mask, step_elems, first, every, last, lane, loaded = -1, entry = 0;
+
+  __device__ __forceinline__ StepWalk(const KvRows& kv, int64_t b, int64_t g, int lane_, int first_, int every_, int last_)
+      : step_elems(kStep * kv.d), first(first_), every(every_), last(last_), lane(lane_) {
+    if (kv.table == nullptr) {
+      table = nullptr;
+      block_elems = 0;
+      base = kv.Row(b, g, 0);
+      shift = 31;
+      mask = 0x7FFFFFFF;
+    } else {
+      table = kv.table + b * kv.stride;
+      block_elems = (static_cast<int64_t>(kv.hkv) << kv.shift) * kv.d;
+      base = (g << kv.shift) * kv.d;
+      shift = kv.shift - 5;
+      mask = (1 << shift) - 1;
+    }
+    num_blocks = static_cast<int32_t>(min(kv.num_blocks, int64_t{0x7FFFFFFF}));
+    stride = kv.stride;
+  }
+  __device__ __forceinline__ int step(int u) const { return min(first + u * every, last); }
+  __device__ __forceinline__ int64_t operator()(int u) {
+    const int t = step(u);
+    if (table == nullptr) return base + static_cast<int64_t>(t) * step_elems;
+    if ((u >> 6) != loaded) {  // (wave-uniform)
+      loaded = u >> 6;
+      const int32_t e = table[min(step((u & ~63) + lane) >> shift, stride - 1)];
+      entry = min(max(e, 0), num_blocks - 1);  // entries outside the pool are clamped into it
+    }
+    return __builtin_amdgcn_readlane(entry, u & 63) * block_elems + base + static_cast<int64_t>(t & mask) * step_elems;
+  }
+};
+
 // Parts of an fp32 value as bf16, largest first: 8 bits each.
 template <int N>
 __device__ __forceinline__ void bf16_parts(float v, __bf16 (&out)[N]) {
@@ -238,7 +277,7 @@ __global__ __launch_bounds__(NW * 64, F32 ? 2 : 4) void kv4_attention_kernel(Att
   uint32_t k_scale[2];      // their scale bytes
   uint32_t v_code[8];       // CW codes of 8 keys
   uint32_t v_scale[2][GR];  // all scale bytes of two runs of 4 keys
-  auto step_rows = [&](int i) { return p.kv.Row(b, g, static_cast<int64_t>(kStep) * (lo + wave + min(i, my - 1) * NW)); };
+  StepWalk step_rows(p.kv, b, g, lane, lo + wave, NW, lo + wave + (my - 1) * NW);
   auto issue_k = [&](int64_t off) {
     const uint8_t* kc = p.kc + off / 2;
     const uint8_t* ks = p.ks + off / 32;
@@ -271,7 +310,9 @@ __global__ __launch_bounds__(NW * 64, F32 ? 2 : 4) void kv4_attention_kernel(Att
   if (my > 0) {
     const int64_t off = step_rows(0);
     issue_k(off);
+    __builtin_amdgcn_sched_barrier(0);  // (in the loop's order: its waits count on the worse one)
     issue_v(off);
+    __builtin_amdgcn_sched_barrier(0);
   }
   for (int i = 0; i < my; ++i) {
     const int64_t next = step_rows(i + 1);
@@ -612,43 +653,6 @@ __device__ __forceinline__ int v_slot(int key, int s) {
   return s ^ (4 * (SL == 16 ? key & 3 : (key >> 1) & 1));
 }
 
-// Row offsets of the 32-key tiles of (b, g), in elements: KvRows::Row of key 32 t without a
-// load that would wait among the LDS reads.  A lane holds one of 64 block-table entries; planes
-// are one block without end.
-struct TileWalk {
-  const int32_t* table;
-  int64_t block_elems, base;
-  int32_t num_blocks, stride, tile_shift, tile_mask, loaded = -1, entry = 0, lane, tile_elems;
-
-  __device__ __forceinline__ TileWalk(const KvRows& kv, int64_t b, int64_t g, int lane_) : lane(lane_), tile_elems(kStep * kv.d) {
-    if (kv.table == nullptr) {
-      table = nullptr;
-      block_elems = 0;
-      base = kv.Row(b, g, 0);
-      tile_shift = 31;
-      tile_mask = 0x7FFFFFFF;
-      loaded = 0;
-    } else {
-      table = kv.table + b * kv.stride;
-      block_elems = (static_cast<int64_t>(kv.hkv) << kv.shift) * kv.d;
-      base = (g << kv.shift) * kv.d;
-      tile_shift = kv.shift - 5;
-      tile_mask = (1 << tile_shift) - 1;
-    }
-    num_blocks = static_cast<int32_t>(min(kv.num_blocks, int64_t{0x7FFFFFFF}));
-    stride = kv.stride;
-  }
-  __device__ __forceinline__ int64_t operator()(int t) {
-    const int blk = t >> tile_shift;
-    if ((blk >> 6) != loaded) {  // (wave-uniform)
-      loaded = blk >> 6;
-      const int32_t e = table[min((blk & ~63) + lane, stride - 1)];
-      entry = min(max(e, 0), num_blocks - 1);  // entries outside the pool are clamped into it
-    }
-    return __builtin_amdgcn_readlane(entry, blk & 63) * block_elems + base + static_cast<int64_t>(t & tile_mask) * tile_elems;
-  }
-};
-
 template <int D, bool F32>
 __global__ __launch_bounds__(512) void kv4_attention_wide_kernel(Attn4Args p) {
   constexpr int QW = kWideWaves, KS = 2;              // waves of a key group, key groups
@@ -728,8 +732,7 @@ __global__ __launch_bounds__(512) void kv4_attention_wide_kernel(Attn4Args p) {
   // which waits for it)
   uint32_t code[NP], scale[NP];
   auto scale_byte = [&](int c) { return (scale[c] >> (8 * ((piece_key(c) * GR + psl / 4) & 3))) & 0xFFu; };
-  TileWalk walk(p.kv, b, g, lane);
-  auto tile_off = [&](int t) { return walk(min(t, ntiles - 1)); };
+  StepWalk tile_off(p.kv, b, g, lane, kg, KS, ntiles - 1);
   const uint32_t code_at = static_cast<uint32_t>(pkey0 * (D / 2) + 4 * psl);
   const uint32_t scale_at = static_cast<uint32_t>((pkey0 * GR + psl / 4) & ~3);
   auto load_tile = [&](int64_t off) {
@@ -752,8 +755,8 @@ __global__ __launch_bounds__(512) void kv4_attention_wide_kernel(Attn4Args p) {
   const int nu = (ntiles + KS - 1) / KS;
   int64_t next_off = 0;
   if (nu > 0) {
-    load_tile(tile_off(kg));
-    next_off = tile_off(kg + KS);
+    load_tile(tile_off(0));
+    next_off = tile_off(1);
   }
 
   // the block's scales of V: the largest, the smallest (but for 0, the scale of zeros) and the first
@@ -1005,7 +1008,7 @@ __global__ __launch_bounds__(512) void kv4_attention_wide_kernel(Attn4Args p) {
     auto load_next = [&](int u) {
       if (u < nu) {
         load_tile(next_off);
-        next_off = tile_off((u + 1) * KS + kg);
+        next_off = tile_off(u + 1);
       }
     };
     auto vector_work = [&](int u) {
