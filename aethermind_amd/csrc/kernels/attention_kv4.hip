@@ -17,6 +17,8 @@
 //     them, and byte permutes gather tile t's column.
 //   * bf16 q: the products of scores are exact in fp32 sums, P is split into two bf16 parts
 //     (16 bits).  fp32 q: q and P are three parts each (24 bits).
+//   * Up to eight columns (HALF): they stand twice in the tile, and each copy takes the softmax of one
+//     of the step's two score tiles.
 //   * exp2 with scale * log2(e) in the exponent's fma.  Running maxima are rescaled only when
 //     one grew.
 // Pieces: every block derives the same plan from the contexts (kv4_plan): pieces of at most
@@ -70,6 +72,11 @@ __device__ __forceinline__ float xor_lane(float v, int lane) {
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     return __uint_as_float(lane < 32 ? r[1] : r[0]);
   }
+}
+
+// Value held by lane (lane ^ 8).
+__device__ __forceinline__ float half_row(float v) {
+  return __uint_as_float(static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(__float_as_uint(v)), 0x128, 0xF, 0xF, false)));  // row_ror:8
 }
 
 // Sum over the lanes up to and including this one.
@@ -214,12 +221,13 @@ __device__ __forceinline__ void bf16_parts(float v, __bf16 (&out)[N]) {
 }
 
 // Two 8-wave blocks fit a CU (fp32 q: one): 128 registers a wave.
-template <int D, bool F32, int NW>
+template <int D, bool F32, int NW, bool HALF>
 __global__ __launch_bounds__(NW * 64, F32 ? 2 : 4) void kv4_attention_kernel(Attn4Args p) {
   constexpr int KK = D / 32;            // MFMA k steps of a score tile
   constexpr int CW = D / 16;            // dimensions per lane of a V row = output tiles
   constexpr int GR = D / 32;            // scale groups of a row
   constexpr int QP = F32 ? 3 : 1, PP = F32 ? 3 : 2;  // bf16 parts of q and P
+  constexpr int SN = HALF ? 4 : 8;      // scores of a lane
   constexpr int NT = NW * 64;
   constexpr int RH = D + 4;             // floats of a column in a record: m, l, 2 pad, o[D]
   extern __shared__ float smem[];       // per wave: o[columns][D], then m, l [columns]
@@ -243,7 +251,8 @@ __global__ __launch_bounds__(NW * 64, F32 ? 2 : 4) void kv4_attention_kernel(Att
   const int my = hi - lo > wave ? (hi - lo - wave + NW - 1) / NW : 0;  // this wave's steps
 
   // column j: position s0 + j / G, head g G + j % G; columns past the last repeat column 0
-  const int col = j < cols ? j : 0, crow = (col * p.g_inv) >> 16;
+  // (HALF: column j - 8 from the eighth on)
+  const int jc = HALF ? j & 7 : j, col = jc < cols ? jc : 0, crow = (col * p.g_inv) >> 16;
   const int64_t qoff = (static_cast<int64_t>(b * p.seq + s0 + crow) * p.hq + g * p.G + col - crow * p.G) * D + (D / 4) * h;
   const int32_t limit = static_cast<int32_t>(
       min(max(seq_position(p.start[b], s0 + crow + 1), int64_t{0}), static_cast<int64_t>(p.cap)));  // keys of the column
@@ -318,10 +327,10 @@ __global__ __launch_bounds__(NW * 64, F32 ? 2 : 4) void kv4_attention_kernel(Att
     const int64_t next = step_rows(i + 1);
     const int32_t first = kStep * (lo + wave + i * NW);  // key of the step
     const int32_t base = first + 4 * h;                  // of this lane's score (0, 0)
-    float sc[8];
+    f32x4_t acc[2];
 #pragma unroll
     for (int tt = 0; tt < 2; ++tt) {
-      f32x4_t acc = f32x4_t{0.f, 0.f, 0.f, 0.f};
+      acc[tt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
       const float s = e8m0_scale_or_nan(k_scale[tt]);
 #pragma unroll
       for (int kk = 0; kk < KK; ++kk) {
@@ -329,22 +338,26 @@ __global__ __launch_bounds__(NW * 64, F32 ? 2 : 4) void kv4_attention_kernel(Att
         fp4_to_bf16(k_code[tt][kk], s, w);
         const bf16x8_t a = __builtin_bit_cast(bf16x8_t, make_uint4(w[0], w[1], w[2], w[3]));
 #pragma unroll
-        for (int i2 = QP - 1; i2 >= 0; --i2) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, qop[i2][kk], acc, 0, 0, 0);
+        for (int i2 = QP - 1; i2 >= 0; --i2) acc[tt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, qop[i2][kk], acc[tt], 0, 0, 0);
       }
-#pragma unroll
-      for (int r = 0; r < 4; ++r) sc[4 * tt + r] = acc[r];
     }
     __builtin_amdgcn_sched_barrier(0);
     issue_k(next);
     __builtin_amdgcn_sched_barrier(0);
-    if (first + kStep > least) {  // (wave-uniform) some column ends in this step
+    float sc[SN];
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (base + 16 * (e >> 2) + (e & 3) >= limit) sc[e] = -INFINITY;
+    for (int e = 0; e < SN; ++e) sc[e] = HALF ? (j < 8 ? acc[0][e] : acc[1][e]) : acc[e >> 2][e & 3];
+    if (first + kStep > least) {  // (wave-uniform) some column ends in this step
+      int32_t key = base + (HALF ? 16 * (j >> 3) : 0);
+      asm volatile("" : "+v"(key));  // (nothing of this in other steps)
+#pragma unroll
+      for (int e = 0; e < SN; ++e)
+        if (key + 16 * (e >> 2) + (e & 3) >= limit) sc[e] = -INFINITY;
     }
     float bm = sc[0];
 #pragma unroll
-    for (int e = 1; e < 8; ++e) bm = fmaxf(bm, sc[e]);
+    for (int e = 1; e < SN; ++e) bm = fmaxf(bm, sc[e]);
+    if constexpr (HALF) bm = fmaxf(bm, half_row(bm));
     bm = fmaxf(bm, xor_lane<16>(bm, lane));
     bm = fmaxf(bm, xor_lane<32>(bm, lane));
     const float mn = fmaxf(m_run, bm * p.scale);
@@ -364,18 +377,32 @@ __global__ __launch_bounds__(NW * 64, F32 ? 2 : 4) void kv4_attention_kernel(Att
     uint32_t pw[PP][4];
     float sum = 0.0f;
 #pragma unroll
-    for (int e = 0; e < 8; e += 2) {
+    for (int e = 0; e < SN; e += 2) {
       float v0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[e], p.scale, sub));
       float v1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[e + 1], p.scale, sub));
       sum += v0;
       sum += v1;
+      if constexpr (!F32) {  // the first part cut off (a permute; the rounding conversion takes two issues), the second rounded
+        const uint32_t u0 = __float_as_uint(v0), u1 = __float_as_uint(v1);
+        pw[0][e / 2] = __builtin_amdgcn_perm(u1, u0, 0x07060302u);
+        v0 -= __uint_as_float(u0 & 0xFFFF0000u);
+        v1 -= __uint_as_float(u1 & 0xFFFF0000u);
+      }
 #pragma unroll
-      for (int i2 = 0; i2 < PP; ++i2) {
+      for (int i2 = F32 ? 0 : 1; i2 < PP; ++i2) {
         const uint32_t w = __builtin_bit_cast(uint32_t, bf16x2_t{static_cast<__bf16>(v0), static_cast<__bf16>(v1)});
         pw[i2][e / 2] = w;
-        v0 -= __uint_as_float(w << 16);
-        v1 -= __uint_as_float(w & 0xFFFF0000u);
+        if (i2 + 1 < PP) {
+          v0 -= __uint_as_float(w << 16);
+          v1 -= __uint_as_float(w & 0xFFFF0000u);
+        }
       }
+    }
+    if constexpr (HALF) {  // lanes of the first half take the other tile's from the second (whose operand rows are not used)
+#pragma unroll
+      for (int i2 = 0; i2 < PP; ++i2)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) pw[i2][2 + i] = __float_as_uint(half_row(__uint_as_float(pw[i2][i])));
     }
     l_run += sum;
     // V: a NaN value must not reach the product, where the probability 0 of a key behind some
@@ -440,6 +467,7 @@ __global__ __launch_bounds__(NW * 64, F32 ? 2 : 4) void kv4_attention_kernel(Att
     }
   }
   // the waves' states into LDS; column j's sum over its four lane groups
+  if constexpr (HALF) l_run += half_row(l_run);
   l_run += xor_lane<16>(l_run, lane);
   l_run += xor_lane<32>(l_run, lane);
   const int ncol = p.qt * p.G;  // columns of a full unit
@@ -1156,7 +1184,8 @@ void Launch(const Attn4Args& p, hipStream_t s) {
   constexpr int NW = kWaves;
   const int lds = NW * (p.qt * p.G * D + 32) * 4;
   RecordLaunch(static_cast<int64_t>(grid.x) * grid.y, NW * 64, lds, "kv4_attention<%s,d=%d,waves=%d,slots=%d>", F32 ? "f32" : "bf16", D, NW, p.slots);
-  hipLaunchKernelGGL((kv4_attention_kernel<D, F32, NW>), grid, dim3(NW * 64), lds, s, p);
+  if (!F32 && p.qt * p.G <= 8) hipLaunchKernelGGL((kv4_attention_kernel<D, F32, NW, !F32>), grid, dim3(NW * 64), lds, s, p);
+  else hipLaunchKernelGGL((kv4_attention_kernel<D, F32, NW, false>), grid, dim3(NW * 64), lds, s, p);
 }
 
 }  // namespace
