@@ -19,8 +19,8 @@
 //     (16 bits).  fp32 q: q and P are three parts each (24 bits).
 //   * Up to eight columns (HALF): they stand twice in the tile, and each copy takes the softmax of one
 //     of the step's two score tiles.
-//   * exp2 with scale * log2(e) in the exponent's fma.  Running maxima are rescaled only when
-//     one grew.
+//   * exp2 with scale * log2(e) in the exponent's fma.  The running sums are rescaled only when a
+//     score passed its column's reference by 2^4.
 // Pieces: every block derives the same plan from the contexts (kv4_plan): pieces of at most
 // `per` steps, the shortest with which all units fit the grid's slots.  The pieces of a unit
 // write records with device-coherent stores and take a ticket; the last one merges them in
@@ -58,6 +58,10 @@ typedef unsigned int u32x4_t __attribute__((ext_vector_type(4)));
 constexpr int kCpolSc1 = 16;
 constexpr int kRawBufferFlags = 0x00020000;
 constexpr float kLog2e = 1.4426950408889634f;
+// A column's reference m (a maximum that its scores passed by at most kSlack, in log2): P = 2^(s - m - kSlack)
+// stays at most 1, and the accumulators are rescaled when a score passes m + kSlack, seldom after
+// the first steps, instead of with every new maximum.
+constexpr float kSlack = 4.0f;
 constexpr int kStep = 32;              // keys of a step
 constexpr int64_t kTicketBytes = 16384;
 constexpr int64_t kMaxSlotHeads = kTicketBytes / 4;  // slots x kv heads of a planned grid
@@ -361,7 +365,7 @@ __global__ __launch_bounds__(NW * 64, F32 ? 2 : 4) void kv4_attention_kernel(Att
     bm = fmaxf(bm, xor_lane<16>(bm, lane));
     bm = fmaxf(bm, xor_lane<32>(bm, lane));
     const float mn = fmaxf(m_run, bm * p.scale);
-    if (__builtin_amdgcn_ballot_w64(mn > m_run) != 0) {
+    if (__builtin_amdgcn_ballot_w64(mn > m_run + kSlack) != 0) {
       const float cf = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m_run - mn);
       l_run *= cf;
 #pragma unroll
@@ -373,7 +377,7 @@ __global__ __launch_bounds__(NW * 64, F32 ? 2 : 4) void kv4_attention_kernel(Att
       m_run = mn;
     }
     // (a column without a live key subtracts 0: exp2(-inf) is 0)
-    const float sub = m_run == -INFINITY ? 0.0f : -m_run;
+    const float sub = m_run == -INFINITY ? 0.0f : -kSlack - m_run;
     uint32_t pw[PP][4];
     float sum = 0.0f;
 #pragma unroll
@@ -638,8 +642,8 @@ __global__ __launch_bounds__(NW * 64, F32 ? 2 : 4) void kv4_attention_kernel(Att
 //   * bf16 q: P is f16, 11 bits where bf16 has 8 (its rounding is 1/8 of out's own), in one
 //     product instead of the two of a bf16 split.  V is f16 as well: codes times 2^(e - E) with E
 //     the largest scale of the group's 32 dimensions among the block's keys, less 13; the block
-//     reads its keys' scale bytes once beforehand (1/17 of the cache).  P carries 2^14 so that its
-//     small values stay normal (below 2^-28 they are held to 2^-39).  Row sums are those of the
+//     reads its keys' scale bytes once beforehand (1/17 of the cache).  P carries 2^15 so that its
+//     small values stay normal (below 2^-25 of the largest they are held to 2^-36 of it).  Row sums are those of the
 //     rounded P.  Where a group's scales differ by more than 2^16, a value that one row alone sees
 //     could push another row's out of f16: such a block takes bf16 V and P in two bf16 parts (2048
 //     rows at 6144 keys: 386 us for 300).
@@ -656,7 +660,7 @@ typedef __attribute__((ext_vector_type(2))) unsigned short u16x2_t;
 constexpr int kWideWaves = 4;   // waves of columns of a block
 constexpr int kVTop = 140;      // exponent byte of the largest scale of V in f16: 6 * 2^13
 constexpr int kNear = 17;        // f16: the largest scale byte of a group less (the smallest - 1)
-constexpr float kPBias = 14.0f;  // log2 of the factor on P in f16
+constexpr float kPBias = 15.0f;  // log2 of the factor on P in f16
 
 __device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
   return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2_t, a), __builtin_bit_cast(u16x2_t, b)));
@@ -914,7 +918,7 @@ __global__ __launch_bounds__(512) void kv4_attention_wide_kernel(Attn4Args p) {
     const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(bm), __float_as_uint(bm), false, false);
     bm = fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1]));
     const float mn = fmaxf(m_run, bm * p.scale);
-    if (__builtin_amdgcn_ballot_w64(mn > m_run) != 0) {
+    if (__builtin_amdgcn_ballot_w64(mn > m_run + kSlack) != 0) {
       const float cf = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m_run - mn);
       l_run *= cf;
 #pragma unroll
@@ -923,7 +927,7 @@ __global__ __launch_bounds__(512) void kv4_attention_wide_kernel(Attn4Args p) {
         for (int r = 0; r < 16; ++r) o[dt][r] *= cf;
       m_run = mn;
     }
-    const float sub = (H ? kPBias : 0.0f) - (m_run == -INFINITY ? 0.0f : m_run);
+    const float sub = (H ? kPBias : 0.0f) - kSlack - (m_run == -INFINITY ? 0.0f : m_run);
 #pragma unroll
     for (int r = 0; r < 16; r += 2) {
       float v0 = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[r], p.scale, sub));

@@ -412,8 +412,8 @@ am_status_code am_gfx950_kv4_read(const am_gfx950_kv4_read_args* args, void* hip
  * q head h reads kv head h / (hq / hkv), at most 16 q heads per kv head and 65535 query
  * rows; fp32 online softmax and sums.  The products take q as it is (bf16) or as three bf16
  * parts (fp32), and the probabilities as two or three; bf16 calls of many rows may round the
- * probabilities to f16 instead (11 bits where out has 8; below 2^-28 of a row's largest,
- * 2^-39 of it).
+ * probabilities to f16 instead (11 bits where out has 8; below 2^-25 of a row's largest,
+ * 2^-36 of it).
  * Scores of which none exceeds minus infinity give zeros.  A NaN among a row's keys gives
  * NaN (a NaN value only in its own 32 dimensions); what the cache holds past a row's keys
  * does not matter.  q and out are 16-byte aligned.

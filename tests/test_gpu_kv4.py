@@ -447,6 +447,24 @@ def test_attention_scale_and_peaked_scores():
     attention_case(5, 2, 3, 8, 2, 128, 512, [500, 77], scale=3.0, dtype="f32")
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("n,hq,hkv", [(1, 8, 2), (5, 8, 2), (400, 64, 16)])
+@pytest.mark.parametrize("rise", [0.02, 0.12, 0.5, -0.1])
+def test_attention_rising_scores(dtype, n, hq, hkv, rise):
+    """scores that rise (or fall) by `rise` a key, beside noise: every step of keys passes the ones before by little or much"""
+    g, d, cap, start = gen_of(n), 64, 800, 380
+    c = Cache(1, hkv, cap, d, 32)
+    u = randn(g, d).sign()
+    k = u * (torch.arange(cap, device="cuda")[:, None] * rise / d) + randn(g, 1, hkv, cap, d) * 0.05
+    c.put_values("k", k)
+    c.put_values("v", randn(g, 1, hkv, cap, d))
+    q = (u * d**0.5 + randn(g, n, hq, d)).view(n, hq * d).to(DTYPES[dtype][0])
+    out = torch.empty_like(q)
+    R.attend(c, q, out, 1, n, hq, i64(start), R.workspace(1, n, hq, hkv, d, cap), dtype=dtype)
+    want, mag, top = R.attention(q.double().view(1, n, hq, d), c.values("k"), c.values("v"), [start], [n], R.softmax_scale(d))
+    assert ((out.double().view_as(want) - want).abs() <= R.attention_bound(want, mag, top, cap, d, dtype)).all()
+
+
 @pytest.mark.parametrize("n", [1, 4, 40])
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 def test_attention_nan_keys_and_values(n, dtype):
