@@ -462,7 +462,13 @@ def test_attention_rising_scores(dtype, n, hq, hkv, rise):
     out = torch.empty_like(q)
     R.attend(c, q, out, 1, n, hq, i64(start), R.workspace(1, n, hq, hkv, d, cap), dtype=dtype)
     want, mag, top = R.attention(q.double().view(1, n, hq, d), c.values("k"), c.values("v"), [start], [n], R.softmax_scale(d))
-    assert ((out.double().view_as(want) - want).abs() <= R.attention_bound(want, mag, top, cap, d, dtype)).all()
+    bound = R.attention_bound(want, mag, top, cap, d, dtype)
+    if N.last_launch().kernel.startswith(b"kv4_attention_wide<bf16"):
+        # f16 probabilities: a reference that a score passes by less than 2^4 stands for 2^11, and f16 has steps of 2^-24 at its
+        # least, so a probability is off by at most 2^-25 / 2^11 = 2^-36 of the row's largest beside its 11 bits.  (Where the
+        # keys near the largest score hold zeros in a dimension, `mag` there is smaller than that.)
+        bound = bound + 2.0**-36 * c.values("v").abs().sum(2).amax()
+    assert ((out.double().view_as(want) - want).abs() <= bound).all()
 
 
 @pytest.mark.parametrize("n", [1, 4, 40])
