@@ -632,8 +632,8 @@ __global__ __launch_bounds__(NW * 64, F32 ? 2 : 4) void kv4_attention_kernel(Att
 // kv head and walks the keys up to its last row's in tiles of 32, in two key groups of four
 // waves that take every other tile and merge in LDS:
 //   * A group's threads load the codes of a tile two intervals ahead, and convert them into one
-//     of four LDS buffers, K and V row-major with their 16-byte slots XORed by the key, so that
-//     the operand reads meet no bank twice.  A conversion serves all the group's columns.
+//     of four LDS buffers, K and V row-major with padded rows, so that the operand reads meet no
+//     bank twice.  A conversion serves all the group's columns.
 //   * S^T = K Q^T on v_mfma_f32_32x32x16_bf16: lane (j, h) holds column j's scores of keys
 //     8 (r >> 2) + 4 h + (r & 3), and these are the k slots of its P operand in
 //     O^T = V^T P^T: P stays in its lane, and so does the softmax state of column j, whose
@@ -673,22 +673,10 @@ __device__ __forceinline__ uint32_t less_one_u16x2(uint32_t a) {
   return __builtin_bit_cast(uint32_t, static_cast<u16x2_t>(__builtin_bit_cast(u16x2_t, a) - u16x2_t{1, 1}));
 }
 
-// Slot of a tile's row (D values, SL slots of 16 bytes) that holds slot s of key `key`: the 16
-// keys of an operand read of K lie in 16 different slots of the banks' 256 bytes, and so do
-// the 4 keys x 4 slots of half a transposed read of V.
-template <int SL>
-__device__ __forceinline__ int k_slot(int key, int s) {
-  return s ^ (SL == 16 ? key & 15 : (key >> 1) & 7);
-}
-template <int SL>
-__device__ __forceinline__ int v_slot(int key, int s) {
-  return s ^ (4 * (SL == 16 ? key & 3 : (key >> 1) & 1));
-}
-
 template <int D, bool F32>
 __global__ __launch_bounds__(512) void kv4_attention_wide_kernel(Attn4Args p) {
   constexpr int QW = kWideWaves, KS = 2;              // waves of a key group, key groups
-  constexpr int GR = D / 32, SL = D / 8;              // scale groups and 16-byte slots of a row
+  constexpr int GR = D / 32, SL = D / 8;              // scale groups and pieces (8 values) of a row
   constexpr int NT = QW * KS * 64, GT = QW * 64;      // threads of the block, of a key group
   constexpr int PC = kStep * SL;                      // pieces (8 values) of a tile of K, of V
   constexpr int NP = 2 * PC / GT;                     // pieces of a thread per tile
@@ -696,9 +684,13 @@ __global__ __launch_bounds__(512) void kv4_attention_wide_kernel(Attn4Args p) {
   constexpr int DT = D / 32;
   constexpr int OW = DT * 16 + 2;                     // words of a lane's state
   static_assert(PC % GT == 0 && GT % SL == 0, "a thread's pieces are K or V by their number alone");
-  constexpr int kTileBytes = kStep * D * 2;
+  // Rows are padded: the 16 keys of an operand read of K lie 16 bytes apart in the banks' 256, the
+  // 4 keys of half a transposed read of V 64 bytes.  (Against 16-byte slots XORed by the key: one
+  // address for all of a tile's reads, the rest is their immediate offset.)
+  constexpr int KR = 2 * D + 16, VR = 2 * D + 64;     // bytes of a row of K, of V
+  constexpr int kBufBytes = kStep * (KR + VR);
   constexpr int NB = 4;                               // buffers of a key group
-  constexpr int kSmem = std::max(KS * NB * 2 * kTileBytes, (KS - 1) * QW * OW * 256);
+  constexpr int kSmem = std::max(KS * NB * kBufBytes, (KS - 1) * QW * OW * 256);
   static_assert(NT == 512, "two waves per SIMD, one of each half");
   __shared__ __align__(16) uint8_t smem_w[kSmem];     // per key group and buffer: K, V
   __shared__ uint32_t s_top[GR], s_low[GR];           // largest and smallest scale of V
@@ -856,6 +848,9 @@ __global__ __launch_bounds__(512) void kv4_attention_wide_kernel(Attn4Args p) {
       __syncthreads();
     }
   }
+  bool any_nan = false;
+#pragma unroll
+  for (int e = 0; e < GR; ++e) any_nan = any_nan || __builtin_amdgcn_readfirstlane(s_nan[e]) != 0x7FFFFFFF;
   bool near = true;  // (block-uniform) the groups' scales lie close enough for f16
 #pragma unroll
   for (int e = 0; e < GR; ++e) near = near && static_cast<int>(s_top[e]) - static_cast<int>(s_low[e]) <= kNear;
@@ -865,11 +860,12 @@ __global__ __launch_bounds__(512) void kv4_attention_wide_kernel(Attn4Args p) {
   constexpr int PP = H ? 1 : F32 ? 3 : 2;  // parts of P
 
   // (buffer of the group's u-th tile)
-  auto tile_k = [&](int u) { return smem_w + (kg * NB + (u & (NB - 1))) * 2 * kTileBytes; };
-  auto tile_v = [&](int u) { return tile_k(u) + kTileBytes; };
+  auto tile_k = [&](int u) { return smem_w + (kg * NB + (u & (NB - 1))) * kBufBytes; };
+  auto tile_v = [&](int u) { return tile_k(u) + kStep * KR; };
   const int v_add = kVTop - static_cast<int>(s_top[psl / 4]);  // to a V piece's scale byte
   auto store_tile = [&](int u) {
     const int t = u * KS + kg;
+    const bool rare = any_nan || kStep * t + kStep > kend;  // (block-uniform) some V counts as zero
 #pragma unroll
     for (int c = 0; c < NP; ++c) {
       const int key = piece_key(c);
@@ -877,19 +873,24 @@ __global__ __launch_bounds__(512) void kv4_attention_wide_kernel(Attn4Args p) {
       uint32_t w[4];
       if (!piece_is_v(c)) {
         fp4_to_bf16(code[c], e8m0_scale_or_nan(sb), w);
-        *reinterpret_cast<uint4*>(tile_k(u) + key * (2 * D) + 16 * k_slot<SL>(key, psl)) = make_uint4(w[0], w[1], w[2], w[3]);
+        *reinterpret_cast<uint4*>(tile_k(u) + key * KR + 16 * psl) = make_uint4(w[0], w[1], w[2], w[3]);
       } else {
-        const bool dead = (sb >= kScaleNan) | (kStep * t + key >= kend);
+        int e = static_cast<int>(sb);
+        if constexpr (H) e = max(e + v_add, 0);  // (a group of zeros may lie below)
+        if (rare) {
+          asm volatile("" : "+v"(e));
+          if (sb >= kScaleNan || kStep * t + key >= kend) e = 0;
+        }
+        const float s = e8m0_scale(static_cast<uint32_t>(e));
         if constexpr (!H) {
-          fp4_to_bf16(code[c], e8m0_scale(dead ? 0u : sb), w);
+          fp4_to_bf16(code[c], s, w);
         } else {
-          const float s = e8m0_scale(static_cast<uint32_t>(max(static_cast<int>(dead ? 0u : sb) + (dead ? 0 : v_add), 0)));
           w[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(code[c], s, 0));
           w[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(code[c], s, 1));
           w[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(code[c], s, 2));
           w[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(code[c], s, 3));
         }
-        *reinterpret_cast<uint4*>(tile_v(u) + key * (2 * D) + 16 * v_slot<SL>(key, psl)) = make_uint4(w[0], w[1], w[2], w[3]);
+        *reinterpret_cast<uint4*>(tile_v(u) + key * VR + 16 * psl) = make_uint4(w[0], w[1], w[2], w[3]);
       }
     }
   };
@@ -953,13 +954,12 @@ __global__ __launch_bounds__(512) void kv4_attention_wide_kernel(Attn4Args p) {
   // 4 h .. +4, which the 16 lanes of a transposed read bring as 4 keys x 16 dimensions
   const int tkey = 4 * h + ((lane & 15) >> 2), tdim = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
   auto read_v = [&](int u, int c, s16x4_t (&part)[DT][2]) {
-    const uint8_t* vt = tile_v(u);
+    const uint8_t* vt = tile_v(u) + tkey * VR + 2 * tdim;
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
-        const int key = 16 * c + 8 * q + tkey, slot = (32 * dt + tdim) >> 3;
-        const uint8_t* at = vt + key * (2 * D) + 16 * v_slot<SL>(key, slot) + 2 * (tdim & 7);
+        const uint8_t* at = vt + (16 * c + 8 * q) * VR + 64 * dt;
         part[dt][q] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4_t*)(at));
       }
   };
@@ -981,7 +981,7 @@ __global__ __launch_bounds__(512) void kv4_attention_wide_kernel(Attn4Args p) {
     }
   };
   auto read_k = [&](int u, int kk) {
-    return *reinterpret_cast<const bf16x8_t*>(tile_k(u) + j * (2 * D) + 16 * k_slot<SL>(j, 2 * kk + h));
+    return *reinterpret_cast<const bf16x8_t*>(tile_k(u) + j * KR + 16 * h + 32 * kk);
   };
   auto score = [&](int kk, bf16x8_t k) {
 #pragma unroll
