@@ -48,6 +48,7 @@ struct Attn4Args {
   int32_t batch, seq, hq, hkv, G, qt, tiles, units, cap;
   int32_t slots;  // planned grid; 0: one piece per unit
   int32_t min_steps;
+  int32_t split;  // many rows: most pieces of a block's keys
   uint32_t tiles_inv;  // ceil(2^32 / tiles): unit / tiles by a multiplication (below 2^16 units)
   int32_t g_inv;  // ceil(2^16 / G): c / G = (c * g_inv) >> 16 for a column c < 32
   float scale;  // of the scores, times log2(e)
@@ -648,6 +649,8 @@ __global__ __launch_bounds__(NW * 64, F32 ? 2 : 4) void kv4_attention_kernel(Att
 //     could push another row's out of f16: such a block takes bf16 V and P in two bf16 parts (2048
 //     rows at 6144 keys: 386 us for 300).
 //   * fp32 q: three bf16 parts of q and P, bf16 V.
+//   * Few row blocks share the CUs by pieces of their keys (planned on the device, as many as
+//     leave each block a CU): records, ticket and merge as above.
 //   * The same pass over the scales finds the first NaN value of each group; it enters the
 //     products as zero and spoils the columns that see its key at the end.
 // What bounds it: VALU work (a tile costs a wave about 120 instructions, 57 of them the
@@ -658,6 +661,10 @@ typedef __attribute__((ext_vector_type(16))) float f32x16_t;
 typedef __attribute__((ext_vector_type(4))) short s16x4_t;
 typedef __attribute__((ext_vector_type(2))) unsigned short u16x2_t;
 constexpr int kWideWaves = 4;   // waves of columns of a block
+// Tiles of a piece of a block's keys.  A merge costs about what 8 tiles do: 200 rows at 2000 keys
+// (four pieces) 26 us, with at least 32 tiles (two) 33.
+constexpr int kMinTiles = 16;
+constexpr int64_t kMaxSplit = 16;
 constexpr int kVTop = 140;      // exponent byte of the largest scale of V in f16: 6 * 2^13
 constexpr int kNear = 17;        // f16: the largest scale byte of a group less (the smallest - 1)
 constexpr float kPBias = 15.0f;  // log2 of the factor on P in f16
@@ -673,7 +680,7 @@ __device__ __forceinline__ uint32_t less_one_u16x2(uint32_t a) {
   return __builtin_bit_cast(uint32_t, static_cast<u16x2_t>(__builtin_bit_cast(u16x2_t, a) - u16x2_t{1, 1}));
 }
 
-template <int D, bool F32>
+template <int D, bool F32, bool SPLIT>
 __global__ __launch_bounds__(512) void kv4_attention_wide_kernel(Attn4Args p) {
   constexpr int QW = kWideWaves, KS = 2;              // waves of a key group, key groups
   constexpr int GR = D / 32, SL = D / 8;              // scale groups and pieces (8 values) of a row
@@ -695,6 +702,7 @@ __global__ __launch_bounds__(512) void kv4_attention_wide_kernel(Attn4Args p) {
   __shared__ __align__(16) uint8_t smem_w[kSmem];     // per key group and buffer: K, V
   __shared__ uint32_t s_top[GR], s_low[GR];           // largest and smallest scale of V
   __shared__ int32_t s_nan[GR];                       // first key with a NaN value
+  __shared__ bool s_last;
 
   const int kg = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / GT);
   const int tid = static_cast<int>(threadIdx.x) - kg * GT, lane = tid & 63;
@@ -709,8 +717,20 @@ __global__ __launch_bounds__(512) void kv4_attention_wide_kernel(Attn4Args p) {
   auto keys_of = [&](int row) {  // keys of row s0 + row
     return static_cast<int32_t>(min(max(seq_position(p.start[b], s0 + row + 1), int64_t{0}), static_cast<int64_t>(p.cap)));
   };
-  const int32_t kend = keys_of(live - 1);
-  const int ntiles = (kend + kStep - 1) / kStep;
+  // the block's piece: tiles [tlo, thi) of its last row's keys
+  const int all_tiles = (keys_of(live - 1) + kStep - 1) / kStep;
+  int pieces = 1, piece = 0, tlo = 0, thi = all_tiles;
+  int32_t kend = keys_of(live - 1);
+  if constexpr (SPLIT) {
+    pieces = max(min(all_tiles / kMinTiles, p.split), 1);
+    piece = static_cast<int>(blockIdx.z);
+    if (piece >= pieces) return;
+    const int per = ((all_tiles + pieces - 1) / pieces + KS - 1) / KS * KS;
+    tlo = min(piece * per, all_tiles);
+    thi = min(tlo + per, all_tiles);
+    kend = min(kend, kStep * thi);  // (no key of another piece counts)
+  }
+  const int ntiles = thi - tlo;
 
   // column j: position s0 + wave qt + j / G, head g G + j % G; columns behind the live rows
   // repeat the last row
@@ -719,7 +739,7 @@ __global__ __launch_bounds__(512) void kv4_attention_wide_kernel(Attn4Args p) {
   const int row = min(wrow + jrow, live - 1);
   const bool mine = j < p.qt * p.G && wrow + jrow < live;
   const int64_t qrow = (static_cast<int64_t>(b * p.seq + s0 + row) * p.hq + g * p.G + jhead) * D;
-  const int32_t limit = keys_of(row), least = keys_of(wrow);
+  const int32_t limit = min(keys_of(row), kend), least = min(keys_of(wrow), kend);
   bf16x8_t qop[QP][D / 16];
 #pragma unroll
   for (int kk = 0; kk < D / 16; ++kk) {
@@ -756,7 +776,7 @@ __global__ __launch_bounds__(512) void kv4_attention_wide_kernel(Attn4Args p) {
   // which waits for it)
   uint32_t code[NP], scale[NP];
   auto scale_byte = [&](int c) { return (scale[c] >> (8 * ((piece_key(c) * GR + psl / 4) & 3))) & 0xFFu; };
-  StepWalk tile_off(p.kv, b, g, lane, kg, KS, ntiles - 1);
+  StepWalk tile_off(p.kv, b, g, lane, tlo + kg, KS, thi - 1);
   const uint32_t code_at = static_cast<uint32_t>(pkey0 * (D / 2) + 4 * psl);
   const uint32_t scale_at = static_cast<uint32_t>((pkey0 * GR + psl / 4) & ~3);
   auto load_tile = [&](int64_t off) {
@@ -796,7 +816,7 @@ __global__ __launch_bounds__(512) void kv4_attention_wide_kernel(Attn4Args p) {
     constexpr int KW = 4 / GR;          // keys of a word
     auto scan = [&](auto&& each) {      // each(word, its first key)
       for (int i = threadIdx.x; i < ntiles * PS; i += NT) {
-        const int step = i / PS, part = i % PS;
+        const int step = tlo + i / PS, part = i % PS;
         const uint4 v = *reinterpret_cast<const uint4*>(p.vs + p.kv.Row(b, g, static_cast<int64_t>(kStep) * step) / 32 + 16 * part);
         const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
@@ -864,7 +884,7 @@ __global__ __launch_bounds__(512) void kv4_attention_wide_kernel(Attn4Args p) {
   auto tile_v = [&](int u) { return tile_k(u) + kStep * KR; };
   const int v_add = kVTop - static_cast<int>(s_top[psl / 4]);  // to a V piece's scale byte
   auto store_tile = [&](int u) {
-    const int t = u * KS + kg;
+    const int t = tlo + u * KS + kg;
     const bool rare = any_nan || kStep * t + kStep > kend;  // (block-uniform) some V counts as zero
 #pragma unroll
     for (int c = 0; c < NP; ++c) {
@@ -905,7 +925,7 @@ __global__ __launch_bounds__(512) void kv4_attention_wide_kernel(Attn4Args p) {
   f32x16_t acc;                                  // scores
   uint32_t pw[PP][2][4];                         // P operand: parts, chunks of 16 keys
   auto softmax = [&](int u) {
-    const int t = u * KS + kg;
+    const int t = tlo + u * KS + kg;
     if (kStep * t + kStep > least) {  // some column of the wave ends in or before this tile
       asm volatile("");               // (a branch: not selects in every tile)
       const int32_t base = kStep * t + 4 * h;
@@ -1096,42 +1116,111 @@ __global__ __launch_bounds__(512) void kv4_attention_wide_kernel(Attn4Args p) {
       rec[(DT * 16 + 1) * 64] = l_run;
     }
     __syncthreads();
-    if (kg > 0) return;
-    const float m2 = rec[DT * 16 * 64], l2 = rec[(DT * 16 + 1) * 64];
-    const float mn = fmaxf(m_run, m2), top = mn == -INFINITY ? 0.0f : mn;
-    const float f1 = __builtin_amdgcn_exp2f(m_run - top), f2 = __builtin_amdgcn_exp2f(m2 - top);
-    l_run = l_run * f1 + l2 * f2;
+    if (kg > 0 && (!SPLIT || pieces == 1)) return;
+    if (kg == 0) {
+      const float m2 = rec[DT * 16 * 64], l2 = rec[(DT * 16 + 1) * 64];
+      const float mn = fmaxf(m_run, m2), top = mn == -INFINITY ? 0.0f : mn;
+      const float f1 = __builtin_amdgcn_exp2f(m_run - top), f2 = __builtin_amdgcn_exp2f(m2 - top);
+      l_run = l_run * f1 + l2 * f2;
+      m_run = mn;
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt) {
-      __builtin_amdgcn_sched_barrier(0);
+      for (int dt = 0; dt < DT; ++dt) {
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int r = 0; r < 16; ++r) o[dt][r] = o[dt][r] * f1 + rec[(dt * 16 + r) * 64] * f2;
+        for (int r = 0; r < 16; ++r) o[dt][r] = o[dt][r] * f1 + rec[(dt * 16 + r) * 64] * f2;
+      }
     }
   }
-  if (!mine) return;
-  const float inv = l_run == 0.0f ? 0.0f : 1.0f / l_run;
+  // V's units back, and the NaN values
+  auto in_units = [&](int dt, float v) {
+    if constexpr (H) v = __builtin_ldexpf(v, static_cast<int>(s_top[dt]) - kVTop);
+    return s_nan[dt] < limit ? __builtin_nanf("") : v;
+  };
+  auto write_out = [&](int dt, int r4, const f32x4_t& v) {
+    const int64_t to = qrow + 32 * dt + 8 * r4 + 4 * h;
+    if constexpr (F32) {
+      *reinterpret_cast<f32x4_t*>(static_cast<float*>(p.out) + to) = v;
+    } else {
+      const uint32_t w0 = f32_to_bf16_bits(v[0]) | (static_cast<uint32_t>(f32_to_bf16_bits(v[1])) << 16);
+      const uint32_t w1 = f32_to_bf16_bits(v[2]) | (static_cast<uint32_t>(f32_to_bf16_bits(v[3])) << 16);
+      *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + to) = make_uint2(w0, w1);
+    }
+  };
+  if (!SPLIT || pieces == 1) {
+    if (!mine) return;
+    const float inv = l_run == 0.0f ? 0.0f : 1.0f / l_run;
 #pragma unroll
-  for (int dt = 0; dt < DT; ++dt) {
-    const bool bad = s_nan[dt] < limit;
-    const int back = static_cast<int>(s_top[dt]) - kVTop;
+    for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-    for (int r4 = 0; r4 < 4; ++r4) {
-      f32x4_t v;
+      for (int r4 = 0; r4 < 4; ++r4) {
+        f32x4_t v;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        v[e] = o[dt][4 * r4 + e] * inv;
-        if constexpr (H) v[e] = __builtin_ldexpf(v[e], back);
-        if (bad) v[e] = __builtin_nanf("");
+        for (int e = 0; e < 4; ++e) v[e] = in_units(dt, o[dt][4 * r4 + e] * inv);
+        write_out(dt, r4, v);
       }
-      const int64_t to = qrow + 32 * dt + 8 * r4 + 4 * h;
-      if constexpr (F32) {
-        *reinterpret_cast<f32x4_t*>(static_cast<float*>(p.out) + to) = v;
-      } else {
-        const uint32_t w0 = f32_to_bf16_bits(v[0]) | (static_cast<uint32_t>(f32_to_bf16_bits(v[1])) << 16);
-        const uint32_t w1 = f32_to_bf16_bits(v[2]) | (static_cast<uint32_t>(f32_to_bf16_bits(v[3])) << 16);
-        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + to) = make_uint2(w0, w1);
+    return;
+  }
+  // Pieces: records as the other kernel's, a lane's state in 16-byte parts, with the reference
+  // that P = 2^(s - m) has; the last piece's block merges them in order, a key group half of the dimensions.
+  if constexpr (SPLIT) {
+    constexpr int kRecBytes = OW * 64 * 4 * QW;
+    const int slot = unit * p.hkv + g;
+    const __amdgpu_buffer_rsrc_t all = __builtin_amdgcn_make_buffer_rsrc(
+        reinterpret_cast<uint8_t*>(p.part) + static_cast<int64_t>(slot) * p.split * kRecBytes, 0, pieces * kRecBytes, kRawBufferFlags);
+    const int mine_at = wave * OW * 64 * 4 + lane * 16, ml_at = wave * OW * 64 * 4 + DT * 16 * 64 * 4 + lane * 8;
+    if (kg == 0) {
+      const float ref = m_run + (kSlack - (H ? kPBias : 0.0f));
+      __builtin_amdgcn_raw_buffer_store_b64(u32x2_t{__float_as_uint(ref), __float_as_uint(l_run)}, all, piece * kRecBytes + ml_at, 0, kCpolSc1);
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int r4 = 0; r4 < 4; ++r4) {
+          f32x4_t v;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = in_units(dt, o[dt][4 * r4 + e]);
+          __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4_t, v), all, piece * kRecBytes + mine_at + (dt * 4 + r4) * 1024, 0, kCpolSc1);
+        }
+    }
+    __builtin_amdgcn_s_waitcnt(0);  // acknowledged before the ticket
+    __syncthreads();
+    if (threadIdx.x == 0)
+      s_last = __hip_atomic_fetch_add(p.tickets + slot, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == static_cast<unsigned>(pieces - 1);
+    __syncthreads();
+    if (!s_last) return;
+    float top = -INFINITY;
+#pragma unroll 4
+    for (int q = 0; q < pieces; ++q)
+      top = fmaxf(top, __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(all, q * kRecBytes + ml_at, 0, kCpolSc1)));
+    top = top == -INFINITY ? 0.0f : top;
+    constexpr int HD = DT / KS;  // output tiles of a key group
+    f32x4_t acc2[HD * 4];
+    float den = 0.0f;
+#pragma unroll
+    for (int i = 0; i < HD * 4; ++i) acc2[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 2
+    for (int q = 0; q < pieces; ++q) {
+      const u32x2_t ml = __builtin_amdgcn_raw_buffer_load_b64(all, q * kRecBytes + ml_at, 0, kCpolSc1);
+      u32x4_t w[HD * 4];
+#pragma unroll
+      for (int i = 0; i < HD * 4; ++i) w[i] = __builtin_amdgcn_raw_buffer_load_b128(all, q * kRecBytes + mine_at + (kg * HD * 4 + i) * 1024, 0, kCpolSc1);
+      const float f = __builtin_amdgcn_exp2f(__uint_as_float(ml[0]) - top);
+      den = __builtin_fmaf(__uint_as_float(ml[1]), f, den);
+#pragma unroll
+      for (int i = 0; i < HD * 4; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc2[i][e] = __builtin_fmaf(__uint_as_float(w[i][e]), f, acc2[i][e]);
+    }
+    if (mine) {
+      const float inv = den == 0.0f ? 0.0f : 1.0f / den;
+#pragma unroll
+      for (int i = 0; i < HD * 4; ++i) {
+        f32x4_t v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = acc2[i][e] * inv;
+        write_out(kg * HD + i / 4, i % 4, v);
       }
     }
+    if (threadIdx.x == 0) __hip_atomic_store(p.tickets + slot, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
   };
   if constexpr (F32) {
@@ -1153,36 +1242,51 @@ int64_t Slots(int64_t units, int64_t hkv, int64_t capacity) {
   return slots * hkv <= kMaxSlotHeads ? slots : 0;
 }
 
-int64_t WorkspaceBytes(int64_t units, int64_t qt, int64_t G, int64_t hkv, int64_t head_dim, int64_t capacity) {
-  return kTicketBytes + Slots(units, hkv, capacity) * hkv * qt * G * (head_dim + 4) * 4;
+// The kernel for many rows: its blocks and the most pieces of a block's keys that leave a CU to each.
+struct Wide {
+  int64_t tiles, blocks, split;
+};
+Wide WidePlan(int64_t batch, int64_t seq, int64_t G, int64_t hkv) {
+  const int64_t tiles = CeilDiv(seq, kWideWaves * (32 / G)), blocks = batch * tiles * hkv;
+  return {tiles, blocks, std::min(std::max<int64_t>(DeviceCUs() / blocks, 1), kMaxSplit)};
+}
+
+// The kernel for many rows where a sequence fills at least one of its blocks and the blocks make
+// up 3/16 of the CUs.  32 q / 8 kv heads, d = 128 (us, this kernel / the other): 256 blocks (1000 rows at
+// 0) 27 / 39; 128 blocks (512 rows) at 0 18.5 / 19.6, at 6144 75 / 112; 56 blocks (200 rows) at 0
+// 12.5 / 10.3, at 2000 26 / 36, at 5000 39 / 57; 32 blocks (100 rows) at 0 10.6 / 6.9.  fp32 q: 80 blocks
+// (300 rows) at 2048 44 / 52.  16 sequences of one row at 4200-8320 keys (128 blocks of one live
+// column group in eight) 273 / 31.
+bool ManyRows(int64_t batch, int64_t seq, int64_t G, int64_t hkv) {
+  return seq >= kWideWaves * (32 / G) && 16 * WidePlan(batch, seq, G, hkv).blocks >= 3 * DeviceCUs();
+}
+
+int64_t WorkspaceBytes(int64_t batch, int64_t seq, int64_t G, int64_t hkv, int64_t head_dim, int64_t capacity) {
+  if (ManyRows(batch, seq, G, hkv)) {
+    const Wide w = WidePlan(batch, seq, G, hkv);
+    return kTicketBytes + (w.split > 1 ? w.blocks * w.split * kWideWaves * 64 * (head_dim / 2 + 2) * 4 : 0);
+  }
+  const int64_t qt = std::min<int64_t>(16 / G, seq);
+  return kTicketBytes + Slots(batch * CeilDiv(seq, qt), hkv, capacity) * hkv * qt * G * (head_dim + 4) * 4;
 }
 
 template <int D, bool F32>
 void LaunchWide(Attn4Args p, hipStream_t s) {
+  const Wide w = WidePlan(p.batch, p.seq, p.G, p.hkv);
   p.qt = 32 / p.G;
-  p.tiles = static_cast<int32_t>(CeilDiv(p.seq, kWideWaves * p.qt));
+  p.tiles = static_cast<int32_t>(w.tiles);
+  p.split = static_cast<int32_t>(w.split);
   p.units = p.batch * p.tiles;
   p.tiles_inv = static_cast<uint32_t>(CeilDiv(int64_t{1} << 32, p.tiles));
-  const dim3 grid(static_cast<unsigned>(p.hkv), static_cast<unsigned>(p.units));
-  RecordLaunch(static_cast<int64_t>(grid.x) * grid.y, 512, 0, "kv4_attention_wide<%s,d=%d>", F32 ? "f32" : "bf16", D);
-  hipLaunchKernelGGL((kv4_attention_wide_kernel<D, F32>), grid, dim3(512), 0, s, p);
-}
-
-// The kernel for many rows where its blocks occupy enough of the CUs (one each) and a sequence
-// fills at least one: its blocks walk their keys whole, while the other kernel's pieces fill
-// the CUs at any shape.  32 q / 8 kv heads, d = 128 (us, this kernel / the other): 128 blocks (512
-// rows) 18.5 / 19.2, 80 blocks (300 rows) 15 / 12.8, 256 blocks (1000 rows) 29 / 41; 16 sequences of
-// one row at 4200-8320 keys (128 blocks of one live column group in eight) 273 / 31; fp32 q does
-// three products for one here: 128 blocks (512 rows at 2048 keys) 94 / 85.
-template <bool F32>
-bool ManyRows(const Attn4Args& p) {
-  const int64_t rows = kWideWaves * (32 / p.G), blocks = p.batch * CeilDiv(p.seq, rows) * p.hkv, cus = DeviceCUs();
-  return p.seq >= rows && (F32 ? 4 : 2) * blocks >= (F32 ? 3 : 1) * cus;
+  const dim3 grid(static_cast<unsigned>(p.hkv), static_cast<unsigned>(p.units), static_cast<unsigned>(p.split));
+  RecordLaunch(static_cast<int64_t>(grid.x) * grid.y * grid.z, 512, 0, "kv4_attention_wide<%s,d=%d,splits=%d>", F32 ? "f32" : "bf16", D, p.split);
+  if (p.split > 1) hipLaunchKernelGGL((kv4_attention_wide_kernel<D, F32, true>), grid, dim3(512), 0, s, p);
+  else hipLaunchKernelGGL((kv4_attention_wide_kernel<D, F32, false>), grid, dim3(512), 0, s, p);
 }
 
 template <int D, bool F32>
 void Launch(const Attn4Args& p, hipStream_t s) {
-  if (ManyRows<F32>(p)) return LaunchWide<D, F32>(p, s);
+  if (ManyRows(p.batch, p.seq, p.G, p.hkv)) return LaunchWide<D, F32>(p, s);
   // kv head fastest: with 8 kv heads every block of a head runs on one XCD
   const dim3 grid(static_cast<unsigned>(p.hkv), static_cast<unsigned>(p.slots > 0 ? p.slots : p.units));
   constexpr int NW = kWaves;
@@ -1202,8 +1306,7 @@ extern "C" int64_t am_gfx950_kv4_attention_workspace_bytes(int64_t batch, int64_
   if (batch <= 0 || seq <= 0 || hkv <= 0 || hq <= 0 || capacity <= 0 || hq % hkv != 0 || hq / hkv > 16 ||
       batch > kMaxRows || seq > kMaxRows || hkv > 65536 || capacity >= (int64_t{1} << 31))
     return kTicketBytes;  // no call takes these
-  const int64_t G = hq / hkv, qt = std::min<int64_t>(16 / G, seq);
-  return WorkspaceBytes(batch * CeilDiv(seq, qt), qt, G, hkv, head_dim, capacity);
+  return WorkspaceBytes(batch, seq, hq / hkv, hkv, head_dim, capacity);
 }
 
 extern "C" am_status_code am_gfx950_kv4_attention(const am_gfx950_kv4_attention_args* a, void* stream) {
@@ -1227,7 +1330,7 @@ extern "C" am_status_code am_gfx950_kv4_attention(const am_gfx950_kv4_attention_
   if (auto st = CheckStreamDevice(AsStream(stream)); st != AM_STATUS_OK) return st;
   const int64_t G = a->hq / a->hkv, qt = std::min<int64_t>(16 / G, a->seq), tiles = CeilDiv(a->seq, qt), units = a->batch * tiles;
   AM_CHECK_ARG(a->workspace != nullptr && Aligned16(a->workspace) &&
-                   a->workspace_bytes >= WorkspaceBytes(units, qt, G, a->hkv, a->head_dim, a->capacity),
+                   a->workspace_bytes >= WorkspaceBytes(a->batch, a->seq, G, a->hkv, a->head_dim, a->capacity),
                "kv4_attention: workspace missing, unaligned or too small");
   p.q = a->q, p.out = a->out;
   p.kc = a->k_codes, p.ks = a->k_scales, p.vc = a->v_codes, p.vs = a->v_scales;

@@ -555,6 +555,48 @@ def test_attention_many_rows(dtype, hq, hkv, d, b, n, start, lens, block):
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("hq,hkv,d,b,n,start,lens,block", [
+    (64, 16, 64, 1, 100, [2300], None, 32),              # two pieces of four
+    (64, 16, 128, 1, 97, [4181], None, 64),              # four pieces, the last one short
+    (32, 16, 64, 3, 64, [2100, 0, 1100], [64, 33, 0], 0),  # sequences of two, one and no pieces
+    (16, 16, 128, 2, 200, [1990, 980], [200, 7], 32),    # rows on both sides of a further piece
+    (96, 16, 64, 1, 60, [-20], None, 0),                 # no keys for some
+    (64, 16, 64, 1, 128, [6000], None, 0),               # past the cache
+])
+def test_attention_many_rows_in_pieces(dtype, hq, hkv, d, b, n, start, lens, block):
+    cap = 3000 if start == [6000] else max(max(s + n for s in start), 64) + 31
+    attention_case(n, b, n, hq, hkv, d, cap - cap % 32, start, lens=lens, block=block, dtype=dtype)
+    assert N.last_launch().kernel.startswith(b"kv4_attention_wide") and b"splits=1>" not in N.last_launch().kernel
+
+
+@pytest.mark.parametrize("which", ["k", "v"])
+def test_attention_many_rows_in_pieces_nan_and_distant_values(which):
+    """a NaN in one piece's keys and values of 2^40 times the others' in another's"""
+    g, hq, hkv, n, start, cap, d = gen_of(5), 64, 16, 100, 2400, 2528, 64
+    c = Cache(1, hkv, cap, d, 32)
+    k, v = randn(g, 1, hkv, cap, d), randn(g, 1, hkv, cap, d)
+    v[:, 2, 2470, :32] *= 2.0**40
+    c.put_values("k", k)
+    c.put_values("v", v)
+    clean = {m: c.values(m) for m in ("k", "v")}
+    marks = c.whole(which + "s")
+    marks[0, 3, 2450, 1] = 255  # seen by rows 50 and later of kv head 3
+    marks[0, 7, 100, 0] = 254   # by all rows of kv head 7
+    c.put(which + "s", marks)
+    q = randn(g, n, hq * d).to(torch.bfloat16)
+    out, ws = torch.empty_like(q), R.workspace(1, n, hq, hkv, d, cap)
+    R.attend(c, q, out, 1, n, hq, i64(start), ws)
+    assert N.last_launch().kernel.startswith(b"kv4_attention_wide") and not ws[:16384].any()
+    want, mag, top = R.attention(q.double().view(1, n, hq, d), clean["k"], clean["v"], [start], [n], R.softmax_scale(d))
+    bad = torch.zeros(n, hq, d, dtype=torch.bool, device="cuda")
+    bad[50:, 12:16, slice(32, 64) if which == "v" else slice(None)] = True
+    bad[:, 28:32, slice(0, 32) if which == "v" else slice(None)] = True
+    got = out.view(n, hq, d)
+    assert torch.equal(torch.isnan(got), bad)
+    assert (((got.double() - want[0]).abs() <= R.attention_bound(want, mag, top, cap, d, "bf16")[0]) | bad).all()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
 def test_attention_many_rows_spread_values(dtype):
     """values whose scales differ widely between keys and between groups, rows that meet only the small ones"""
     g, n, hq, hkv, d, cap = gen_of(3), 400, 64, 16, 128, 416
