@@ -809,6 +809,42 @@ def test_graphs_that_share_a_workspace():
     assert not ws[:16384].any()
 
 
+def test_graph_of_pieces_beside_decode():
+    """a captured call of many rows in pieces and one of single rows, on one workspace, at other positions in every replay"""
+    g, hq, hkv, d, cap, n = gen_of(31), 64, 16, 64, 4096, 100
+    c = Cache(1, hkv, cap, d, 64)
+    for m in ("k", "v"):
+        c.put_values(m, randn(g, 1, hkv, cap, d))
+    ws = torch.zeros(max(R.workspace(1, r, hq, hkv, d, cap).numel() for r in (n, 1)), dtype=torch.uint8, device="cuda")
+    q = [torch.zeros(r, hq * d, dtype=torch.bfloat16, device="cuda") for r in (n, 1)]
+    out = [torch.zeros_like(t) for t in q]
+    start = [i64(0), i64(0)]
+
+    def step():
+        for x, y, s in zip(q, out, start):
+            R.attend(c, x, y, 1, x.shape[0], hq, s, ws)
+
+    start[0].fill_(2200)
+    step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for first in (3900, 0, 2048, 700):
+        for x in q:
+            x.copy_(randn(g, *x.shape))
+        start[0].fill_(first), start[1].fill_(first + n)
+        for y in out:
+            y.zero_()
+        graph.replay()
+        got = [y.clone() for y in out]
+        torch.cuda.synchronize()
+        for y in out:
+            y.zero_()
+        step()
+        assert all(torch.equal(x, y) for x, y in zip(got, out))
+        assert out[0].any(-1).all() and not ws[:16384].any()
+
+
 def test_other_stream():
     m = Model(2, 8, 2, 64, 256, 32)
     g = gen_of(6)
