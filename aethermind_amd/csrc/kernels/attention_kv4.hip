@@ -883,9 +883,16 @@ __global__ __launch_bounds__(512) void kv4_attention_wide_kernel(Attn4Args p) {
   auto tile_k = [&](int u) { return smem_w + (kg * NB + (u & (NB - 1))) * kBufBytes; };
   auto tile_v = [&](int u) { return tile_k(u) + kStep * KR; };
   const int v_add = kVTop - static_cast<int>(s_top[psl / 4]);  // to a V piece's scale byte
-  auto store_tile = [&](int u) {
+  // V pieces that count as zero: NaN values, and keys past the last
+  auto clear_dead = [&](int u) {
     const int t = tlo + u * KS + kg;
-    const bool rare = any_nan || kStep * t + kStep > kend;  // (block-uniform) some V counts as zero
+    if (any_nan || kStep * t + kStep > kend) {  // (block-uniform)
+#pragma unroll
+      for (int c = NK; c < NP; ++c)
+        if (scale_byte(c) >= kScaleNan || kStep * t + piece_key(c) >= kend) code[c] = scale[c] = 0;
+    }
+  };
+  auto store_tile = [&](int u) {
 #pragma unroll
     for (int c = 0; c < NP; ++c) {
       const int key = piece_key(c);
@@ -897,10 +904,6 @@ __global__ __launch_bounds__(512) void kv4_attention_wide_kernel(Attn4Args p) {
       } else {
         int e = static_cast<int>(sb);
         if constexpr (H) e = max(e + v_add, 0);  // (a group of zeros may lie below)
-        if (rare) {
-          asm volatile("" : "+v"(e));
-          if (sb >= kScaleNan || kStep * t + key >= kend) e = 0;
-        }
         const float s = e8m0_scale(static_cast<uint32_t>(e));
         if constexpr (!H) {
           fp4_to_bf16(code[c], s, w);
@@ -1057,20 +1060,23 @@ __global__ __launch_bounds__(512) void kv4_attention_wide_kernel(Attn4Args p) {
     __builtin_amdgcn_sched_barrier(0);
   };
   if (nu > 0) {
+    // (Tiles past the last are the last one again, into buffers that are free: no branch, so that
+    // the softmax and the staging mix.)
     auto load_next = [&](int u) {
-      if (u < nu) {
-        load_tile(next_off);
-        next_off = tile_off(u + 1);
-      }
+      load_tile(next_off);
+      next_off = tile_off(u + 1);
     };
     auto vector_work = [&](int u) {
+      clear_dead(u + 2);
       softmax(u);
-      if (u + 2 < nu) store_tile(u + 2);
+      store_tile(u + 2);
       load_next(u + 3);
     };
+    clear_dead(0);
     store_tile(0);
     load_next(1);
-    if (nu > 1) store_tile(1);
+    clear_dead(1);
+    store_tile(1);
     load_next(2);
     interval_end();
     read_m(0, false, true);
