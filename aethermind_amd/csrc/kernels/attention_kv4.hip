@@ -26,6 +26,13 @@
 // write records with device-coherent stores and take a ticket; the last one merges them in
 // piece order, so results do not depend on the schedule.  (The ordering that this relies on,
 // relaxed device-coherent accesses around a wait, is the one of attention.hip's merge.)
+//
+// What bounds it (32 q / 8 kv heads, d = 128, bf16, us inside a graph): one token over 131072 keys (143 MB)
+// 33.5, 4.3 TB/s; the same kernel without its arithmetic 32.2, without its loads 25.8.  A plain read of
+// those bytes takes 24 with its launch (2), so the fixed part is the rest: the plan and the first load (2), the waves'
+// merge, record and ticket (3), the last block's merge (3).  16 sequences at 4200-8320 keys,
+// paged (111 MB) 29 (27, 24); one at 640 keys 6.7 (5.1, 6.5: a step's chain of conversion, product,
+// softmax, product is its latency).
 
 #include <algorithm>
 #include <cmath>
@@ -647,14 +654,16 @@ __global__ __launch_bounds__(NW * 64, F32 ? 2 : 4) void kv4_attention_kernel(Att
 //     small values stay normal (below 2^-25 of the largest they are held to 2^-36 of it).  Row sums are those of the
 //     rounded P.  Where a group's scales differ by more than 2^16, a value that one row alone sees
 //     could push another row's out of f16: such a block takes bf16 V and P in two bf16 parts (2048
-//     rows at 6144 keys: 386 us for 300).
+//     rows at 6144 keys: 331 us for 261).
 //   * fp32 q: three bf16 parts of q and P, bf16 V.
 //   * Few row blocks share the CUs by pieces of their keys (planned on the device, as many as
 //     leave each block a CU): records, ticket and merge as above.
 //   * The same pass over the scales finds the first NaN value of each group; it enters the
 //     products as zero and spoils the columns that see its key at the end.
-// What bounds it: VALU work (a tile costs a wave about 120 instructions, 57 of them the
-// softmax's, beside 16 MFMAs), which the MFMAs of the SIMD's other wave hide.
+// What bounds it: 2048 rows at 6144 keys take 261 us, 0.92 PFLOP/s; the matrix pipes are busy 36% of
+// that, the VALU 45%, LDS 32%, and a wave waits a third of its time to issue or at barriers.  Without the
+// staging (conversion and LDS writes) it takes 221, without the products with V 252, without the
+// exponentials 253, without the operand reads 253.
 typedef __attribute__((ext_vector_type(8))) _Float16 f16x8_t;
 typedef __attribute__((ext_vector_type(2))) _Float16 f16x2_t;
 typedef __attribute__((ext_vector_type(16))) float f32x16_t;
@@ -1049,7 +1058,7 @@ __global__ __launch_bounds__(512) void kv4_attention_wide_kernel(Attn4Args p) {
   // of the staging) and products (M: P V of tile u, K Q^T of tile u + 1).  Between two barriers
   // the first group does V then M, and the second, which shares every SIMD with it, M (of the
   // tile before) then V: while one wave of a SIMD multiplies the other exponentiates.  In phase
-  // (every wave V then M, a barrier a tile) 2048 rows at 6144 keys took 329 us, so 300.
+  // (every wave V then M, a barrier a tile) 2048 rows at 6144 keys took 329 us, so 300 at the time.
   // Interval u stores tile u + 2.  K of tile x is read in interval x - 1 (ahead of x in the
   // second group), its V in x or x + 1: four buffers.
   // (kg as a lane value: as a scalar one the loops' registers spill)
