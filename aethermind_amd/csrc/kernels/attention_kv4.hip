@@ -685,6 +685,20 @@ __device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
 __device__ __forceinline__ uint32_t min_u16x2(uint32_t a, uint32_t b) {
   return __builtin_bit_cast(uint32_t, __builtin_elementwise_min(__builtin_bit_cast(u16x2_t, a), __builtin_bit_cast(u16x2_t, b)));
 }
+// Lane 63: op over all lanes.
+template <class F>
+__device__ __forceinline__ uint32_t wave_last(uint32_t v, F op) {
+  auto with = [&]<int CTRL, int ROWS>() {
+    v = op(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(static_cast<int>(v), static_cast<int>(v), CTRL, ROWS, 0xF, false)));
+  };
+  with.template operator()<0x111, 0xF>();
+  with.template operator()<0x112, 0xF>();
+  with.template operator()<0x114, 0xF>();
+  with.template operator()<0x118, 0xF>();
+  with.template operator()<0x142, 0xA>();
+  with.template operator()<0x143, 0xC>();
+  return v;
+}
 __device__ __forceinline__ uint32_t less_one_u16x2(uint32_t a) {
   return __builtin_bit_cast(uint32_t, static_cast<u16x2_t>(__builtin_bit_cast(u16x2_t, a) - u16x2_t{1, 1}));
 }
@@ -846,13 +860,11 @@ __global__ __launch_bounds__(512) void kv4_attention_wide_kernel(Attn4Args p) {
       }
     });
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int o = 32; o > 0; o >>= 1) {
-        top[i] = max_u16x2(top[i], static_cast<uint32_t>(__shfl_xor(static_cast<int>(top[i]), o)));
-        low[i] = min_u16x2(low[i], static_cast<uint32_t>(__shfl_xor(static_cast<int>(low[i]), o)));
-      }
-    if (lane == 0) {
+    for (int i = 0; i < 2; ++i) {
+      top[i] = wave_last(top[i], [](uint32_t a, uint32_t b) { return max_u16x2(a, b); });
+      low[i] = wave_last(low[i], [](uint32_t a, uint32_t b) { return min_u16x2(a, b); });
+    }
+    if (lane == 63) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         atomicMax(&s_top[e % GR], (top[e & 1] >> (8 * (e & 2))) & 0xFFFFu);
