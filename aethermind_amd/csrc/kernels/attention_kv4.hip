@@ -169,7 +169,8 @@ __device__ __forceinline__ Piece kv4_plan(const Attn4Args& p, int slot, int lane
     if (at < all) {
       const int i = __builtin_popcountll(__builtin_amdgcn_ballot_w64(upto <= at));
       const int mine = __builtin_amdgcn_readlane(n, i), before = __builtin_amdgcn_readlane(upto, i) - mine;
-      return {c + i, at - before, mine, slot - (at - before), mine == 1 ? kWholeSteps + hi : hi};
+      const int steps = __builtin_amdgcn_readlane(st, i);  // (in equal pieces of at most hi)
+      return {c + i, at - before, mine, slot - (at - before), mine == 1 ? kWholeSteps + hi : (steps + mine - 1) / mine};
     }
     at -= all;
   }
