@@ -55,6 +55,7 @@ struct Attn4Args {
   int32_t batch, seq, hq, hkv, G, qt, tiles, units, cap;
   int32_t slots;  // planned grid; 0: one piece per unit
   int32_t min_steps;
+  int32_t few_slots, few_steps;  // slots for at most few_steps steps in all
   int32_t split;  // many rows: most pieces of a block's keys
   uint32_t tiles_inv;  // ceil(2^32 / tiles): unit / tiles by a multiplication (below 2^16 units)
   int32_t g_inv;  // ceil(2^16 / G): c / G = (c * g_inv) >> 16 for a column c < 32
@@ -126,6 +127,7 @@ __device__ __forceinline__ int unit_steps(const Attn4Args& p, int u) {
 // kMinSteps.
 constexpr int kWholeSteps = 32;
 constexpr int kMinSteps = 16;
+constexpr int kFewSteps = 32;  // of a CU
 
 // Which unit and piece the slot takes.  per: steps of a piece.  unit < 0: no work.
 struct Piece {
@@ -155,10 +157,11 @@ __device__ __forceinline__ Piece kv4_plan(const Attn4Args& p, int slot, int lane
     return n;
   };
   // ceil(steps / per) summed over the units is at most total / per + units, so `hi` fits
-  int lo = max((total + p.slots - 1) / p.slots, p.min_steps);
-  int hi = max((total + p.slots - p.units - 1) / (p.slots - p.units), lo);
+  const int slots = total <= p.few_steps ? p.few_slots : p.slots;
+  int lo = max((total + slots - 1) / slots, p.min_steps);
+  int hi = max((total + slots - p.units - 1) / (slots - p.units), lo);
   for (int mid = lo; lo < hi; mid = (lo + hi) >> 1) {  // (equal contexts mostly fit at the first try)
-    if (pieces_at(mid) <= p.slots) hi = mid;
+    if (pieces_at(mid) <= slots) hi = mid;
     else lo = mid + 1;
   }
   int at = slot;
@@ -1371,6 +1374,12 @@ extern "C" am_status_code am_gfx950_kv4_attention(const am_gfx950_kv4_attention_
   p.cap = static_cast<int32_t>(a->capacity);
   p.slots = static_cast<int32_t>(Slots(units, a->hkv, a->capacity));
   p.min_steps = kMinSteps;
+  // Little work runs in one block a CU: a second one's merges cost more than it takes over.
+  // 8 sequences at 1500-3000 keys (17 steps a CU) 14.3 -> 12.5 us, at 2500-5000 (29) 15.3 -> 14.2, 16 at
+  // 1500-3000 (35) the same either way.
+  const int64_t cus = DeviceCUs(), few = CeilDiv(cus, a->hkv);
+  p.few_slots = static_cast<int32_t>(few >= 2 * units ? std::min<int64_t>(few, p.slots) : p.slots);
+  p.few_steps = static_cast<int32_t>(kFewSteps * cus / a->hkv);
   p.tiles_inv = static_cast<uint32_t>(CeilDiv(int64_t{1} << 32, tiles));
   p.g_inv = static_cast<int32_t>(CeilDiv(1 << 16, G));
   p.scale = kLog2e * (a->scale > 0.0f ? a->scale : 1.0f / sqrtf(static_cast<float>(a->head_dim)));
