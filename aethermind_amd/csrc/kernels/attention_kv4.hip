@@ -113,9 +113,10 @@ __device__ __forceinline__ int unit_seq(const Attn4Args& p, int u) {
 // Keys of the unit's last live row, in [0, cap]; rows: its live rows (may be 0).
 __device__ __forceinline__ int32_t unit_keys(const Attn4Args& p, int u, int32_t& rows) {
   const int b = unit_seq(p, u), s0 = (u - b * p.tiles) * p.qt;
+  const int64_t start = p.start[b];  // (in flight beside the length)
   rows = min(live_rows(p.lens, b, p.seq) - s0, p.qt);
   if (rows <= 0) return 0;
-  const int64_t n = seq_position(p.start[b], s0 + rows);
+  const int64_t n = seq_position(start, s0 + rows);
   return static_cast<int32_t>(min(max(n, int64_t{0}), static_cast<int64_t>(p.cap)));
 }
 __device__ __forceinline__ int unit_steps(const Attn4Args& p, int u) {

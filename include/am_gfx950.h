@@ -418,10 +418,11 @@ am_status_code am_gfx950_kv4_read(const am_gfx950_kv4_read_args* args, void* hip
  * NaN (a NaN value only in its own 32 dimensions); what the cache holds past a row's keys
  * does not matter.  q and out are 16-byte aligned.
  * workspace: am_gfx950_kv4_attention_workspace_bytes(...) bytes, 16-byte aligned, whose
- * first 16384 bytes must be zero before the first call and are left zero.  One workspace
- * serves this function's calls of any shapes in turn (not am_gfx950_attention's, whose
- * records would reach into those bytes); calls that overlap on one workspace race.  Equal
- * calls give equal bits. */
+ * first 16384 bytes must be zero before the first call and are left zero.  One workspace of
+ * the largest size that its calls need (not always the one of most rows) serves this
+ * function's calls of any shapes in turn (not am_gfx950_attention's, whose records would
+ * reach into those bytes); calls that overlap on one workspace race.  Equal calls give
+ * equal bits. */
 typedef struct am_gfx950_kv4_attention_args {
   const void* q;
   void* out;
