@@ -473,9 +473,9 @@ __global__ __launch_bounds__(NW * 64, F32 ? 2 : 4) void kv4_attention_kernel(Att
   }
 
   // NaN values: the columns that have the key, in its group's dimensions
-  nan_key = min(nan_key, __shfl_xor(nan_key, 16));
-  nan_key = min(nan_key, __shfl_xor(nan_key, 32));
   if (__builtin_amdgcn_ballot_w64(nan_key != 0x7FFFFFFF) != 0) {
+    nan_key = min(nan_key, __shfl_xor(nan_key, 16));
+    nan_key = min(nan_key, __shfl_xor(nan_key, 32));
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const bool bad = nan_key < __shfl(limit, 16 * h + 4 * h + r);
