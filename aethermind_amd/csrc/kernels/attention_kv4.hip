@@ -379,13 +379,15 @@ __global__ __launch_bounds__(NW * 64, F32 ? 2 : 4) void kv4_attention_kernel(Att
     bm = fmaxf(bm, xor_lane<32>(bm, lane));
     const float mn = fmaxf(m_run, bm * p.scale);
     if (__builtin_amdgcn_ballot_w64(mn > m_run + kSlack) != 0) {
-      const float cf = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m_run - mn);
-      l_run *= cf;
+      if (__builtin_amdgcn_ballot_w64(m_run > -INFINITY) != 0) {  // (nothing to rescale before the first scores)
+        const float cf = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m_run - mn);
+        l_run *= cf;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const float cr = __shfl(cf, 16 * h + 4 * h + r);
+        for (int r = 0; r < 4; ++r) {
+          const float cr = __shfl(cf, 16 * h + 4 * h + r);
 #pragma unroll
-        for (int t = 0; t < CW; ++t) o[t][r] *= cr;
+          for (int t = 0; t < CW; ++t) o[t][r] *= cr;
+        }
       }
       m_run = mn;
     }
