@@ -31,7 +31,7 @@
 // 33.5, 4.3 TB/s; the same kernel without its arithmetic 32.2, without its loads 25.8.  A plain read of
 // those bytes takes 24 with its launch (2), so the fixed part is the rest: the plan and the first load (2), the waves'
 // merge, record and ticket (3), the last block's merge (3).  16 sequences at 4200-8320 keys,
-// paged (111 MB) 29 (27, 24); one at 640 keys 6.7 (5.1, 6.5: a step's chain of conversion, product,
+// paged (111 MB) 28.8 (27, 24); one at 640 keys 6.5 (5.1, 6.4: a step's chain of conversion, product,
 // softmax, product is its latency).
 
 #include <algorithm>
