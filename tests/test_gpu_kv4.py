@@ -888,3 +888,17 @@ def test_two_streams_at_once():
     for m, ws, want in zip(models, spaces, alone):
         assert torch.equal(m.out, want)
         assert not ws[:16384].any()
+
+
+@pytest.mark.parametrize("n", [1, 100, 400])
+def test_attention_refuses_a_smaller_workspace(n):
+    """single rows over many keys, many rows in pieces, many rows: 16 bytes less than the size asked for"""
+    hq, hkv, d, cap = 64, 16, 64, 4096
+    c = Cache(1, hkv, cap, d, fill=0, scale_fill=0)
+    q = torch.zeros(n, hq * d, dtype=torch.bfloat16, device="cuda")
+    out, ws = torch.full_like(q, 2.0), R.workspace(1, n, hq, hkv, d, cap)
+    with pytest.raises(N.NativeError):
+        R.attend(c, q, out, 1, n, hq, i64(cap - n), ws[:-16])
+    assert (out == 2.0).all()
+    R.attend(c, q, out, 1, n, hq, i64(cap - n), ws)
+    assert (out == 0.0).all()
